@@ -1,0 +1,239 @@
+// Rows in 8-bit integers with a 32-bit scale per row, the operands of linear_int8.cu:
+//
+//   scales[r] = max_c |y[r, c]| / 127,     out[r, c] = the whole number nearest to y[r, c] / scales[r] (ties to even)
+//
+// of three kinds of rows y, formed in 32-bit and rounded only here:
+//   rows as they are                       (a weight's rows, an attention's output)
+//   act(gate) * up of rows [gate | up]     (a gated feed-forward)
+//   s * rsqrt(mean(s^2) + eps) * w         (RMSNorm) with s = x (+ residual), residual <- round(s)
+//
+// The norm needs one pass: y = rstd * (s w) with rstd the same for the whole row, so max|y| = rstd max|s w| and the whole numbers are
+// those of s w, which the statistics do not enter.  Sum of squares and maximum come out of the same reduction (one barrier).
+//
+// Rounding: s w * (127 / max) + 1.5 * 2^23 in one fused multiply-add leaves the nearest whole number, ties to even, in the sum's low
+// bits (two's complement); |s w * (127 / max)| is at most 127 (1 + 2^-23), which is 127 again.  A row whose maximum is below 2^-90 is
+// multiplied by 2^100 first, so that 127 / max stays finite.  A row of zeros gets the scale 0 (the norm's formula: NaN where eps is 0
+// too).  A row that holds an infinity or a NaN has no scale: it gets the scale NaN and zeros, so that everything made of it is NaN and
+// the other rows are untouched.  (The maximum is taken of the bit patterns of |y|, in whose order infinities and then NaN come last.)
+//
+// The work is bound by memory.  A block takes a row and holds it in registers between the reduction and the store (PER groups of VEC
+// neighbouring elements per thread, all loads in flight together); rows too long for that are read a second time.
+#include "common.cuh"
+
+#define RQ_PLAIN 0
+#define RQ_ACT 1
+#define RQ_NORM 2
+
+struct RqParams {
+  const void* x;          // rows of `cols` (RQ_ACT: 2 * cols) elements
+  void* residual;         // RQ_NORM: [rows, cols] or null, updated in place
+  const float* weight;    // RQ_NORM: [cols]
+  signed char* out;       // [rows, cols]
+  float* scales;          // [rows]
+  long long x_stride, out_stride;  // elements between rows (residual: cols)
+  int cols;
+  int act;                // RQ_ACT: 0 silu, 1 gelu_tanh
+  float eps;
+};
+
+// a gate's activation without a branch: g / (1 + e^-z).  The fast quotient is 0 for a denominator beyond 2^126, where the true value is
+// below 2^-119.
+__device__ __forceinline__ float rq_gate(float g, int act) {
+  const float z = act == 0 ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
+  return __fdividef(g, 1.f + expf(-z));
+}
+
+// (sum, largest bit pattern) over the block, the same in every thread; the order of additions depends on blockDim alone
+__device__ __forceinline__ void rq_reduce(float& sum, uint32_t& top, bool with_sum) {
+  __shared__ float sums[32];
+  __shared__ uint32_t tops[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (with_sum) sum = warp_sum(sum);
+  if (warps == 1) return;
+  if (lane == 0) tops[warp] = top, sums[warp] = sum;
+  __syncthreads();
+  top = __reduce_max_sync(0xffffffffu, lane < warps ? tops[lane] : 0u);
+  if (with_sum) sum = warp_sum(lane < warps ? sums[lane] : 0.f);
+}
+
+struct RqRow {
+  float pre, mul;   // out = round(v * pre * mul)
+  uint32_t keep;    // all ones, or 0 for a row that is not finite
+  float scale;
+};
+__device__ __forceinline__ RqRow rq_row(uint32_t top, float rstd) {
+  RqRow r;
+  const float most = __uint_as_float(top);
+  r.pre = most < 8.077935669463161e-28f ? 1.2676506002282294e30f : 1.f;  // 2^-90, 2^100
+  r.mul = top == 0u ? 0.f : 127.f / (most * r.pre);
+  r.keep = top < 0x7f800000u ? 0xffffffffu : 0u;
+  r.scale = r.keep ? rstd * most / 127.f : __uint_as_float(0x7fc00000u);
+  return r;
+}
+__device__ __forceinline__ uint32_t rq_round(const RqRow& r, float v) {
+  return __float_as_uint(fmaf(v * r.pre, r.mul, 12582912.f)) & r.keep;
+}
+
+// VEC values of one place of a row; RQ_NORM: unrounded sums in s beside v = s * w
+template <typename T, int KIND, int VEC>
+__device__ __forceinline__ void rq_load(const RqParams& p, const T* x, const T* res, int c, float (&v)[VEC], float (&s)[VEC]) {
+  load_vec<T, VEC>(x + c, v);
+  if constexpr (KIND == RQ_ACT) {
+    load_vec<T, VEC>(x + p.cols + c, s);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = rq_gate(v[i], p.act) * s[i];
+  }
+  if constexpr (KIND == RQ_NORM) {
+    if (res != nullptr) {
+      load_vec<T, VEC>(res + c, s);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s[i] += v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s[i] = v[i];
+    }
+    load_vec32<VEC>(p.weight + c, v);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] *= s[i];
+  }
+}
+template <int KIND, int VEC>
+__device__ __forceinline__ void rq_account(const float (&v)[VEC], const float (&s)[VEC], float& sum, uint32_t& top) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    if (KIND == RQ_NORM) sum = fmaf(s[i], s[i], sum);
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void rq_store(const RqRow& r, signed char* out, const float (&v)[VEC]) {
+  uint32_t q[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) q[i] = rq_round(r, v[i]);
+  if constexpr (VEC % 4 == 0) {
+    uint32_t w[VEC / 4];
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i)
+      w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410);
+    if constexpr (VEC == 8)
+      *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+    else
+      *reinterpret_cast<uint32_t*>(out) = w[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[i] = (signed char)(q[i] & 0xff);
+  }
+}
+
+// PER > 0: the row in registers, PER * VEC * blockDim >= cols.  PER = 0: any length, read twice.
+template <typename T, int KIND, int VEC, int PER>
+__global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long row = blockIdx.x;
+  const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_stride;
+  T* res = KIND == RQ_NORM && p.residual != nullptr ? reinterpret_cast<T*>(p.residual) + row * p.cols : nullptr;
+  signed char* out = p.out + row * p.out_stride;
+  constexpr int P = PER > 0 ? PER : 1;
+  float v[P][VEC], s[P][VEC];
+  float sum = 0.f;
+  uint32_t top = 0u;
+  if constexpr (PER > 0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = (i * blockDim.x + threadIdx.x) * VEC;
+      if (c < p.cols) {
+        rq_load<T, KIND, VEC>(p, x, res, c, v[i], s[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[i][e] = s[i][e] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      rq_account<KIND, VEC>(v[i], s[i], sum, top);
+      const int c = (i * blockDim.x + threadIdx.x) * VEC;
+      if (KIND == RQ_NORM && res != nullptr && c < p.cols) store_vec<T, VEC>(res + c, s[i]);
+    }
+  } else {
+    for (int c = threadIdx.x * VEC; c < p.cols; c += blockDim.x * VEC) {
+      rq_load<T, KIND, VEC>(p, x, res, c, v[0], s[0]);
+      rq_account<KIND, VEC>(v[0], s[0], sum, top);
+    }
+  }
+  rq_reduce(sum, top, KIND == RQ_NORM);
+  const RqRow r = rq_row(top, KIND == RQ_NORM ? rsqrtf(sum / (float)p.cols + p.eps) : 1.f);
+  if (threadIdx.x == 0) p.scales[row] = r.scale;
+  if constexpr (PER > 0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = (i * blockDim.x + threadIdx.x) * VEC;
+      if (c < p.cols) rq_store<VEC>(r, out + c, v[i]);
+    }
+  } else {
+    for (int c = threadIdx.x * VEC; c < p.cols; c += blockDim.x * VEC) {
+      rq_load<T, KIND, VEC>(p, x, res, c, v[0], s[0]);
+      if (KIND == RQ_NORM && res != nullptr) store_vec<T, VEC>(res + c, s[0]);
+      rq_store<VEC>(r, out + c, v[0]);
+    }
+  }
+}
+
+template <typename T, int KIND, int VEC>
+static int rq_launch_vec(const RqParams& p, int rows, cudaStream_t st) {
+  const int groups = (p.cols + VEC - 1) / VEC;
+  auto go = [&](auto kernel, int per) {
+    int threads = ((groups + per - 1) / per + 31) / 32 * 32;
+    return ullm_launch_kernel(kernel, dim3(rows), dim3(threads > 1024 ? 1024 : threads), 0, st, p);
+  };
+  if (groups <= 1024) return go(rows_int8_kernel<T, KIND, VEC, 1>, 1);
+  if (groups <= 2048) return go(rows_int8_kernel<T, KIND, VEC, 2>, 2);
+  if (groups <= 4096) return go(rows_int8_kernel<T, KIND, VEC, 4>, 4);
+  return go(rows_int8_kernel<T, KIND, VEC, 0>, 4);
+}
+
+template <typename T, int KIND>
+static int rq_launch(const RqParams& p, int rows, cudaStream_t st) {
+  constexpr int V = 16 / (int)sizeof(T);
+  // 16-byte pieces of every input row, V bytes of every output row
+  const bool wide = p.cols % V == 0 && (uintptr_t)p.x % 16 == 0 && p.x_stride % V == 0 && (uintptr_t)p.residual % 16 == 0 &&
+                    (uintptr_t)p.weight % 16 == 0 && (uintptr_t)p.out % V == 0 && p.out_stride % V == 0;
+  return wide ? rq_launch_vec<T, KIND, V>(p, rows, st) : rq_launch_vec<T, KIND, 1>(p, rows, st);
+}
+
+template <int KIND>
+static int rq_run(int dtype, const RqParams& p, int rows, void* stream) {
+  if (rows < 0 || p.cols <= 0 || p.cols > (1 << 28) || p.out_stride < p.cols || p.x_stride < p.cols) return ULLM_ERR_BAD_SIZE;
+  if (dtype != ULLM_DTYPE_F32 && dtype != ULLM_DTYPE_BF16 && dtype != ULLM_DTYPE_F16) return ULLM_ERR_BAD_DTYPE;
+  if (rows == 0) return ULLM_OK;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == ULLM_DTYPE_F32) return rq_launch<float, KIND>(p, rows, st);
+  if (dtype == ULLM_DTYPE_BF16) return rq_launch<__nv_bfloat16, KIND>(p, rows, st);
+  return rq_launch<__half, KIND>(p, rows, st);
+}
+
+// Strides in elements.
+extern "C" int ullm_quantize_rows_int8(int dtype, const void* x, long long x_stride, void* out, long long out_stride, void* scales,
+                                       int rows, int cols, void* stream) {
+  RqParams p = {};
+  p.x = x, p.x_stride = x_stride, p.out = (signed char*)out, p.out_stride = out_stride, p.scales = (float*)scales, p.cols = cols;
+  return rq_run<RQ_PLAIN>(dtype, p, rows, stream);
+}
+
+extern "C" int ullm_act_mul_int8(int dtype, int act, const void* gate_up, void* out, long long out_stride, void* scales, int rows,
+                                 int inter, void* stream) {
+  if (act != 0 && act != 1) return ULLM_ERR_BAD_SIZE;
+  RqParams p = {};
+  p.x = gate_up, p.x_stride = 2ll * inter, p.out = (signed char*)out, p.out_stride = out_stride, p.scales = (float*)scales;
+  p.cols = inter, p.act = act;
+  return rq_run<RQ_ACT>(dtype, p, rows, stream);
+}
+
+extern "C" int ullm_add_rmsnorm_int8(int dtype, const void* x, void* residual, const void* weight, void* out, long long out_stride,
+                                     void* scales, int rows, int cols, float eps, void* stream) {
+  RqParams p = {};
+  p.x = x, p.x_stride = cols, p.residual = residual, p.weight = (const float*)weight, p.out = (signed char*)out;
+  p.out_stride = out_stride, p.scales = (float*)scales, p.cols = cols, p.eps = eps;
+  return rq_run<RQ_NORM>(dtype, p, rows, stream);
+}
