@@ -151,7 +151,17 @@ def run(x, xs, w, ws, dtype, bias=None):
 # products whose tiles are shared by 1 to 8 blocks
 PRODUCTS = [(1, 1, 16), (1, 6144, 4096), (2, 128, 128), (7, 130, 144), (8, 24576, 1024), (16, 1000, 4096), (17, 257, 400),
             (32, 4096, 2048), (33, 384, 1040), (64, 4096, 12288), (65, 500, 272), (127, 129, 2064), (128, 6144, 1024), (129, 1030, 656),
-            (200, 2048, 2048), (256, 640, 512), (257, 1000, 784), (511, 4096, 256), (1000, 2500, 528), (2048, 4096, 4096)]
+            (200, 2048, 2048), (256, 640, 512), (257, 1000, 784), (511, 4096, 256), (1000, 2500, 528), (2048, 4096, 4096),
+            (16, 7156, 5232), (13, 2000, 8208), (16, 6144, 2064), (20, 300, 2064), (30, 2000, 8208), (31, 6100, 2064), (31, 6683, 7072), (32, 12300, 1040),
+            (61, 5000, 2064), (40, 520, 2064), (64, 10000, 528), (100, 24500, 272), (97, 4666, 4320), (125, 6100, 2064), (300, 4090, 2064),
+            (333, 12200, 1040), (120, 2393, 5856), (513, 6200, 1040), (2047, 4095, 272), (700, 20001, 400)]
+
+
+def test_the_products_take_every_form():
+    """(1,000 x blocks that share a tile + its tokens; negative: pairs of blocks.  148 SMs, which the choice goes by.)"""
+    if torch.cuda.get_device_properties(0).multi_processor_count == 148:
+        forms = {K().lib.ullm_linear_int8_form(*p) for p in PRODUCTS}
+        assert forms >= {1016, 2016, 4016, 8016, 1032, 2032, 4032, 8032, 1064, 2064, 4064, 1128, 2128, 4128, -256}, forms
 
 
 @pytest.mark.parametrize("M,N,k", PRODUCTS)

@@ -5,9 +5,11 @@
 // a product is cut does not show in its result.  The result is formed in float32, times x_scales first, and rounded once.  A token whose
 // scale is NaN (a row that had no finite maximum) has NaN results; no other token's change.
 //
-// Two kernels:
-//   linear_int8_tc      the tcgen05 tensor cores (kind::i8), operands by TMA: rows on borders of 16 bytes.  See there.
-//   linear_int8_plain   anything else: rows at any address, four products an instruction (dp4a).
+// Three kernels:
+//   linear_int8_tc      the tcgen05 tensor cores (kind::i8), operands by TMA (rows on borders of 16 bytes): few tokens, narrow products;
+//   linear_int8_pair    the same for many tokens, two SMs to a tile;
+//   linear_int8_plain   rows at any address, four products an instruction (dp4a).
+// `li_choose` says which of the first two takes a product.
 #include "tcgen05_util.cuh"
 
 #define LI_MAX_K 131071
@@ -28,6 +30,27 @@ struct LiParams {
 template <typename T>
 __device__ __forceinline__ T li_result(int sum, float xs, float ws, float bias) {
   return from_f32<T>(fmaf((float)sum * xs, ws, bias));
+}
+
+// One channel of W tokens, of which `tokens` exist: out[i * stride] = result of v[i].  All scales are read before the first store,
+// which the compiler could not move them in front of (out might be anywhere): 64 columns end in 0.6 us instead of 2.
+template <typename T, int W>
+__device__ __forceinline__ void li_store(T* out, int stride, const int (&v)[W], const float* xs, float ws, float bias, int tokens) {
+  T r[W];
+#pragma unroll
+  for (int i = 0; i < W; i += 4) {
+    const float4 s = *reinterpret_cast<const float4*>(xs + i);
+    r[i] = li_result<T>(v[i], s.x, ws, bias), r[i + 1] = li_result<T>(v[i + 1], s.y, ws, bias);
+    r[i + 2] = li_result<T>(v[i + 2], s.z, ws, bias), r[i + 3] = li_result<T>(v[i + 3], s.w, ws, bias);
+  }
+  if (tokens >= W) {
+#pragma unroll
+    for (int i = 0; i < W; ++i, out += stride) *out = r[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i, out += stride)
+      if (i < tokens) *out = r[i];
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -77,7 +100,7 @@ __global__ void __launch_bounds__(256) linear_int8_plain(const LiParams p) {
 
 // ---------------------------------------------------------------------------------------------
 // The tensor cores.  A tile is 128 channels by NT tokens: channels are the instruction's M (the lanes of tensor memory), tokens its N
-// (16 to 256), so that few tokens cost few columns and every weight byte still meets a full instruction.  A block of six warps:
+// (16 to 128), so that few tokens cost few columns and every weight byte still meets a full instruction.  A block of six warps:
 //   warp 0 (one lane)  TMA loads of 128 k of both operands (128-byte swizzle) into a ring of stages;
 //   warp 1             tcgen05.mma, 32 k an instruction, the accumulator (32-bit whole numbers) in tensor memory;
 //   warps 2 to 5       the end: a thread owns a channel; a warp stores 32 neighbouring channels of a token at a time.
@@ -136,6 +159,7 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
   __shared__ __align__(8) uint64_t full_bar[LI_MAX_STAGES], empty_bar[LI_MAX_STAGES], acc_bar;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
+  __shared__ __align__(16) float xs_s[NT + 32];  // the tile's token scales
   unsigned char* ring = (unsigned char*)(((uintptr_t)li_smem_raw + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)blockIdx.x % p.ksplit, n0 = (int)blockIdx.x / p.ksplit * 128;
@@ -214,7 +238,11 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
   const int n = n0 + chan;
   const uint32_t taddr = tmem_d + ((uint32_t)(quarter * 32) << 16);
   T* out = reinterpret_cast<T*>(p.out);
+  const float ws = warp >= 2 && n < p.N ? p.w_scales[n] : 0.f;
+  const float bias = warp >= 2 && n < p.N && p.bias != nullptr ? to_f32(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
   if (warp >= 2) {
+    for (int i = threadIdx.x - 64; i < tokens; i += 128) xs_s[i] = p.x_scales[m0 + i];
+    asm volatile("bar.sync 1, 128;" ::: "memory");
     ok = __all_sync(0xffffffffu, mbar_wait(&acc_bar, 0));
     if (!ok) {
       if (lane == 0) ullm_report(p.status, ULLM_STATUS_TIMEOUT, 133, 0);
@@ -222,44 +250,54 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
     }
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   }
-  const float ws = warp >= 2 && n < p.N ? p.w_scales[n] : 0.f;
-  const float bias = warp >= 2 && n < p.N && p.bias != nullptr ? to_f32(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
   if (p.ksplit == 1) {
     if (warp >= 2 && ok) {
       for (int c = 0; c < tokens; c += 16) {
         int v[16];
         li_tmem_ld16(taddr + c, v);
-        if (n < p.N) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (c + i < tokens) out[(size_t)(m0 + c + i) * p.N + n] = li_result<T>(v[i], p.x_scales[m0 + c + i], ws, bias);
-        }
+        if (n < p.N) li_store<T, 16>(out + (size_t)(m0 + c) * p.N + n, p.N, v, xs_s + c, ws, bias, tokens - c);
       }
     }
   } else {
-    const int share = (tokens + p.ksplit - 1) / p.ksplit;  // tokens that a block finishes
+    // tokens that a block finishes, a multiple of 4: the sums travel as [block they come from][quad of tokens][channel][4 tokens]
+    const int share = ((tokens + p.ksplit - 1) / p.ksplit + 3) & ~3;
     li_cluster_sync();  // every block's ring is drained (its accumulator is complete) or given up
     if (warp >= 2 && ok) {
+      const uint32_t mine = lin_smem(ring) + (uint32_t)((rank * (share >> 2)) * 128 + chan) * 16;
+      int to = 0, at = 0;  // the block that the next quad goes to, the quad's place there
+      uint32_t dst = li_rank_addr(mine, 0);
       for (int c = 0; c < tokens; c += 16) {
         int v[16];
         li_tmem_ld16(taddr + c, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (c + i >= tokens) break;
-          const int to = (c + i) / share, at = (c + i) - to * share;
-          const uint32_t dst = li_rank_addr(lin_smem(ring) + (uint32_t)(((rank * share + at) * 128 + chan) * 4), (uint32_t)to);
-          asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(dst), "r"(v[i]) : "memory");
+        for (int i = 0; i < 16; i += 4) {
+          if (c + i < tokens)
+            asm volatile("st.shared::cluster.v4.s32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (uint32_t)at * 2048u), "r"(v[i]), "r"(v[i + 1]),
+                         "r"(v[i + 2]), "r"(v[i + 3])
+                         : "memory");
+          if (++at == share >> 2) at = 0, dst = li_rank_addr(mine, (uint32_t)min(++to, p.ksplit - 1));
         }
       }
     }
     li_cluster_sync();
     if (warp >= 2 && ok && n < p.N) {
-      const int* got = reinterpret_cast<const int*>(ring);
-      for (int t = 0; t < share && rank * share + t < tokens; ++t) {
-        int sum = 0;
-        for (int r = 0; r < p.ksplit; ++r) sum += got[(r * share + t) * 128 + chan];
-        const int m = m0 + rank * share + t;
-        out[(size_t)m * p.N + n] = li_result<T>(sum, p.x_scales[m], ws, bias);
+      constexpr int W = NT < 32 ? 4 : 16;  // tokens at a time: their loads run beside one another
+      const int4* got = reinterpret_cast<const int4*>(ring) + chan;
+      const int mine_end = min(share, tokens - rank * share);
+      for (int t = 0; t < mine_end; t += W) {
+        int v[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = 0;
+        for (int r = 0; r < p.ksplit; ++r) {
+#pragma unroll
+          for (int i = 0; i < W; i += 4) {
+            if (t + i >= share) break;
+            const int4 q = got[(r * (share >> 2) + ((t + i) >> 2)) * 128];
+            v[i] += q.x, v[i + 1] += q.y, v[i + 2] += q.z, v[i + 3] += q.w;
+          }
+        }
+        const int m = rank * share + t;
+        li_store<T, W>(out + (size_t)(m0 + m) * p.N + n, p.N, v, xs_s + m, ws, bias, mine_end - t);
       }
     }
   }
@@ -275,6 +313,213 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
   }
 }
 
+// ---------------------------------------------------------------------------------------------
+// Many tokens.  Two blocks (a cluster of two SMs of one pair, cta_group::2) make tiles of 256 channels by 256 tokens: each holds 128 of
+// the channels and half of the tokens in shared memory, the leader's instructions read both halves, and each block's tensor memory
+// takes its own 128 channels.  So a block loads 32 KB for the work that takes 48 KB alone, which is what keeps the tensor cores fed
+// from L2.  Persistent: tiles go round the clusters, tokens fastest (the weights then come from memory once), and
+// two accumulators let a tile's end run beside the next one's products.
+//
+// Barriers: a stage is full when the bytes of both blocks have come (the leader's barrier counts them all); an instruction group's
+// commit frees the stage in both blocks, and tells both that an accumulator is complete; the eight finishing warps of both tell the
+// leader that it is drained.
+// ---------------------------------------------------------------------------------------------
+#define LI_PAIR_STAGES 6
+#define LI_PAIR_TOKENS 256
+
+__device__ __forceinline__ void li_pair_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void li_pair_mma(uint32_t lead, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %0, 0;\n"
+      " @q tcgen05.mma.cta_group::2.kind::i8 [%1], %2, %3, %4, p;\n}\n"
+      ::"r"(lead), "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// arrives at the barrier of this address in both blocks when the instructions so far are done
+__device__ __forceinline__ void li_pair_commit(uint32_t lead, uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n .reg .b16 both;\n setp.ne.b32 q, %0, 0;\n mov.b16 both, 3;\n"
+      " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%1], both;\n}\n"
+      ::"r"(lead), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void li_arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ bool li_wait_cluster(uint64_t* bar, uint32_t parity) {
+  for (int i = 0; i < WAIT_LIMIT; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(lin_smem(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ void li_tmem_ld32(uint32_t taddr, int (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+      "%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+        "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+        "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LI_THREADS)
+linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const LiParams p) {
+  constexpr int BN = LI_PAIR_TOKENS, STAGE = LI_W_BYTES + BN / 2 * 128;
+  extern __shared__ unsigned char li_smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[LI_PAIR_STAGES], empty_bar[LI_PAIR_STAGES], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag, go[2];
+  __shared__ __align__(16) float xs_s[2][BN];  // the token scales of a tile
+  unsigned char* ring = (unsigned char*)(((uintptr_t)li_smem_raw + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)blockIdx.x & 1, cluster = (int)blockIdx.x >> 1, clusters = (int)gridDim.x >> 1;
+  const int t_tiles = (p.M + BN - 1) / BN;
+  const long long tiles = (long long)t_tiles * ((p.N + 255) / 256);
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < LI_PAIR_STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 8);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lin_smem(&tmem_slot)), "r"(2 * BN)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    pdl_launch_dependents();  // (only now: a kernel behind this one must not hold tensor memory that this one waits for)
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  li_cluster_sync();  // the other block's barriers exist
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_d = tmem_slot;
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t parity = 1;  // a fresh barrier passes a wait on parity 1
+      bool ok = true;
+      for (long long tile = cluster; tile < tiles && ok; tile += clusters) {
+        const int c0 = (int)(tile / t_tiles) * 256 + rank * 128, t0 = (int)(tile % t_tiles) * BN + rank * (BN / 2);
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!mbar_wait(&empty_bar[s], parity)) {
+            ullm_report(p.status, ULLM_STATUS_TIMEOUT, 134, kb);
+            abort_flag = 1;
+            ok = false;
+            break;
+          }
+          const uint32_t bar = li_rank_addr(lin_smem(&full_bar[s]), 0), st = lin_smem(ring + s * STAGE);
+          if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * STAGE);
+          li_pair_load(st, &w_map, bar, kb * 128, c0);
+          li_pair_load(st + LI_W_BYTES, &x_map, bar, kb * 128, t0);
+          if (++s == LI_PAIR_STAGES) s = 0, parity ^= 1;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0) {
+      constexpr uint32_t idesc = li_idesc(256, BN);
+      const uint32_t lead = elect_one();
+      const uint64_t desc0 = umma_desc(ring);
+      int s = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (long long tile = cluster; tile < tiles && ok; tile += clusters, ++it) {
+        const int buf = it & 1;
+        if (!__all_sync(0xffffffffu, li_wait_cluster(&acc_empty[buf], ((it >> 1) & 1) ^ 1))) {
+          if (lane == 0) ullm_report(p.status, ULLM_STATUS_TIMEOUT, 135, it);
+          abort_flag = 1;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d = tmem_d + (uint32_t)(buf * BN);
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[s], phase))) {
+            if (lane == 0) ullm_report(p.status, ULLM_STATUS_TIMEOUT, 136, kb);
+            abort_flag = 1;
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint64_t a = desc0 + (uint64_t)(s * (STAGE >> 4)), b = a + (LI_W_BYTES >> 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) li_pair_mma(lead, d, a + 2 * j, b + 2 * j, idesc, kb > 0 || j > 0);
+          li_pair_commit(lead, lin_smem(&empty_bar[s]));
+          if (++s == LI_PAIR_STAGES) s = 0, phase ^= 1;
+        }
+        if (ok) li_pair_commit(lead, lin_smem(&acc_full[buf]));
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    int it = 0;
+    for (long long tile = cluster; tile < tiles; tile += clusters, ++it) {
+      const int buf = it & 1;
+      const int n = (int)(tile / t_tiles) * 256 + rank * 128 + quarter * 32 + lane, m0 = (int)(tile % t_tiles) * BN;
+      const int tokens = min(BN, p.M - m0);
+      for (int i = threadIdx.x - 64; i < BN; i += 128) xs_s[buf][i] = i < tokens ? p.x_scales[m0 + i] : 0.f;
+      const float ws = n < p.N ? p.w_scales[n] : 0.f;
+      const float bias = n < p.N && p.bias != nullptr ? to_f32(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
+      // one thread waits (bounded) and tells the others, so that all 128 take the same way out
+      if (threadIdx.x == 64) {
+        const bool got = mbar_wait(&acc_full[buf], (it >> 1) & 1);
+        if (!got) ullm_report(p.status, ULLM_STATUS_TIMEOUT, 137, it), abort_flag = 1;
+        go[buf] = got;
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (!go[buf]) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t taddr = tmem_d + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN);
+      T* out = reinterpret_cast<T*>(p.out) + (size_t)m0 * p.N + n;
+      for (int c = 0; c < tokens; c += 32) {
+        int v[32];
+        li_tmem_ld32(taddr + c, v);
+        if (n < p.N) li_store<T, 32>(out + (size_t)c * p.N, p.N, v, xs_s[buf] + c, ws, bias, tokens - c);
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) li_arrive_at(li_rank_addr(lin_smem(&acc_empty[buf]), 0));
+    }
+  }
+  __syncthreads();
+  if (abort_flag && rank == 0 && threadIdx.x == 0) {
+    // a wait ran out: copies may still be on their way into either block's ring, whose bytes the leader's barriers count
+    const long long mine = tiles > cluster ? ((tiles - 1 - cluster) / clusters + 1) * p.k_blocks : 0;
+    for (int s = 0; s < LI_PAIR_STAGES && s < mine; ++s) mbar_wait(&full_bar[s], (uint32_t)((mine - 1 - s) / LI_PAIR_STAGES) & 1);
+  }
+  __syncthreads();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  li_cluster_sync();  // nobody arrives at this block's barriers any more, or reads its ring
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_d), "r"(2 * BN) : "memory");
+  }
+}
+
 // rows of 8-bit numbers, boxes of box_rows x 128 bytes
 static bool li_map(const void* ptr, long long rows, long long cols, long long stride, int box_rows, CUtensorMap* out) {
   EncodeTiledFn enc = get_encode();
@@ -287,29 +532,75 @@ static bool li_map(const void* ptr, long long rows, long long cols, long long st
 
 static int g_li_sms = 0;
 
+// Clusters of `ks` blocks that a product of tiles of `nt` tokens is given at most: so many that their blocks come to 4/3 of the SMs, two on
+// some; where a block takes a whole SM, what finds room at once (a GPC's SMs are no multiple of a cluster: 32 clusters of 4 do, 34 take
+// a second round, 96 x 2,057 x 1,104 in 8.6 us for 5.4).
+static int li_clusters_most(int nt, int ks) {
+  if (nt < 64) return 4 * g_li_sms / (3 * ks);
+  return ks == 2 ? g_li_sms * 36 / 74 : ks == 4 ? g_li_sms * 16 / 74 : 0;
+}
+
+// Which form a product takes: the one that this estimate finds fastest, in ns.  A launch and a tile's end take `start`; a stage of 128 k
+// takes `one` where an SM has one block at a time and `two` where it has two; weights come from memory at 6.4 GB a ms at most (5 through
+// pairs).  Sharing tiles costs two meetings of the cluster and the way of the sums.  The constants are fitted to 247 products (1 to
+// 2,048 tokens, 320 to 24,576 channels, k of 512 to 12,288), each timed in every form: the form chosen here takes 0.7 % more than the
+// fastest one on average, 11 % at most.  What the forms are for, in us beside the nearest alternative:
+//   16, 32, 64 tokens a tile   few tokens: 8 x 24,576 x 4,096 19.8; 64 x 4,096 x 12,288 12.7 (pairs 31)
+//   shared tiles               few tiles: 8 x 4,096 x 4,096 5.8 (alone 9.7), 8 x 2,048 x 8,192 6.0 (alone 16.8)
+//   128 tokens a tile          96 x 24,576 x 4,096 22.7 (64 tokens 31, pairs 27); 384 x 12,288 x 4,096 18.6 (28; 26)
+//   pairs, 256 tokens          512 x 24,576 x 4,096 39 (128 tokens 65); 2,048 x 24,576 x 4,096 128 (248)
+struct LiForm {
+  int pair, tile, ksplit;
+};
+static LiForm li_choose(int M, int N, int K) {
+  static const int tile[4] = {16, 32, 64, 128}, start[4] = {2700, 2800, 3500, 4000}, one[4] = {250, 240, 260, 270},
+                   two[4] = {400, 300, 365, 465};
+  const int k_blocks = (K + 127) / 128;
+  const long long sms = g_li_sms;
+  const double weights = (double)N * K;
+  LiForm best = {0, 16, 1};
+  double least = 1e300;
+  for (int i = 0; i < 4; ++i) {
+    const int nt = tile[i];
+    if ((i > 0 && nt >= 2 * M) || (nt < 64 && nt < M)) continue;
+    const long long tiles = (long long)((N + 127) / 128) * ((M + nt - 1) / nt);
+    for (int ks = 1; ks <= 8; ks *= 2) {
+      if (ks > 1 && (k_blocks < 2 * ks || tiles > li_clusters_most(nt, ks))) break;
+      const long long blocks = tiles * ks, rounds = blocks / (2 * sms), rest = blocks % (2 * sms);
+      const double stage = (double)rounds * two[i] + (rest == 0 ? 0 : rest <= sms ? one[i] : two[i]);
+      double t = stage * ((k_blocks + ks - 1) / ks);
+      if (t < weights / 6400) t = weights / 6400;
+      t += start[i] + (ks > 1 ? 160 + 24 * (nt < M ? nt : M) : 0);
+      if (t < least) least = t, best = {0, nt, ks};
+    }
+  }
+  if (M > 64) {
+    const long long tiles = (long long)((N + 255) / 256) * ((M + LI_PAIR_TOKENS - 1) / LI_PAIR_TOKENS);
+    double t = (double)((tiles + sms / 2 - 1) / (sms / 2)) * k_blocks * 277;
+    if (t < weights / 5000) t = weights / 5000;
+    if (t + 5680 < least) best = {1, LI_PAIR_TOKENS, 1};
+  }
+  return best;
+}
+
 template <typename T, int NT>
-static int li_launch_tc(LiParams p, cudaStream_t st) {
+static int li_launch_tc(LiParams p, int ksplit, cudaStream_t st) {
   constexpr int STAGE = LI_W_BYTES + NT * 128;
-  constexpr int PER_SM = NT <= 64 ? 2 : 1;
-  constexpr int STAGES_MOST = ((PER_SM == 2 ? 110 : 216) * 1024 - 1024) / STAGE;
-  constexpr int STAGES = STAGES_MOST < LI_MAX_STAGES ? STAGES_MOST : LI_MAX_STAGES;
-  static_assert(STAGES * STAGE >= (NT + 8) * 512, "the ring holds a cluster's sums");
-  const int smem = STAGES * STAGE + 1024;
+  // Two blocks an SM, or one with a ring of up to 12 stages: where an SM has one block only, and where two rings would be too short.
+  constexpr int DEEP = 216 * 1024 / STAGE < LI_MAX_STAGES ? 216 * 1024 / STAGE : LI_MAX_STAGES, HALF = 109 * 1024 / STAGE;
+  static_assert((NT < 64 ? HALF : DEEP) * STAGE >= (NT + 32) * 512, "the ring holds a cluster's sums");
+  const int n_tiles = (p.N + 127) / 128, m_tiles = (p.M + NT - 1) / NT;
+  if (m_tiles > 65535) return ULLM_ERR_UNSUPPORTED;
   static bool set = false;
   if (!set) {
-    if (cudaFuncSetAttribute(linear_int8_tc<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    if (cudaFuncSetAttribute(linear_int8_tc<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, DEEP * STAGE + 1024) != cudaSuccess)
       return ULLM_ERR_LAUNCH;
     set = true;
   }
-  const int n_tiles = (p.N + 127) / 128, m_tiles = (p.M + NT - 1) / NT;
-  if (m_tiles > 65535) return ULLM_ERR_UNSUPPORTED;
-  const long long tiles = (long long)n_tiles * m_tiles;
-  int ksplit = (int)(PER_SM * g_li_sms / tiles);
-  if (ksplit > 8) ksplit = 8;
-  if (ksplit > p.k_blocks / 2) ksplit = p.k_blocks / 2;
-  if (ksplit < 1) ksplit = 1;
   p.ksplit = ksplit;
-  p.stages = STAGES;
+  const long long blocks = (long long)n_tiles * m_tiles * ksplit;
+  p.stages = NT >= 64 && (ksplit > 1 || blocks <= g_li_sms) ? DEEP : HALF;
+  const int smem = p.stages * STAGE + 1024;
   CUtensorMap w_map, x_map;
   if (!li_map(p.w, p.N, p.K, p.w_stride, 128, &w_map) || !li_map(p.x, p.M, p.K, p.x_stride, NT, &x_map)) return ULLM_ERR_LAUNCH;
   cudaLaunchConfig_t cfg = {};
@@ -333,17 +624,50 @@ static int li_launch_tc(LiParams p, cudaStream_t st) {
 }
 
 template <typename T>
+static int li_launch_pair(const LiParams& p, cudaStream_t st) {
+  constexpr int BN = LI_PAIR_TOKENS;
+  const int smem = LI_PAIR_STAGES * (LI_W_BYTES + BN / 2 * 128) + 1024;
+  static bool set = false;
+  if (!set) {
+    if (cudaFuncSetAttribute(linear_int8_pair<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      return ULLM_ERR_LAUNCH;
+    set = true;
+  }
+  const long long tiles = (long long)((p.M + BN - 1) / BN) * ((p.N + 255) / 256);
+  const int clusters = (int)(tiles < g_li_sms / 2 ? tiles : g_li_sms / 2);
+  CUtensorMap w_map, x_map;
+  if (!li_map(p.w, p.N, p.K, p.w_stride, 128, &w_map) || !li_map(p.x, p.M, p.K, p.x_stride, BN / 2, &x_map)) return ULLM_ERR_LAUNCH;
+  return ullm_launch_kernel(linear_int8_pair<T>, dim3(2 * clusters), dim3(LI_THREADS), smem, st, w_map, x_map, p);
+}
+
+template <typename T>
 static int li_run(const LiParams& p, cudaStream_t st) {
   const bool aligned = (((uintptr_t)p.x | (uintptr_t)p.w | (uintptr_t)p.x_stride | (uintptr_t)p.w_stride) & 15) == 0;
   if (!aligned) {
     if ((p.M + 31ll) / 32 > 65535) return ULLM_ERR_UNSUPPORTED;
     return ullm_launch_kernel(linear_int8_plain<T>, dim3((p.N + 31) / 32, (p.M + 31) / 32), dim3(256), 0, st, p);
   }
-  if (p.M <= 16) return li_launch_tc<T, 16>(p, st);
-  if (p.M <= 32) return li_launch_tc<T, 32>(p, st);
-  if (p.M <= 64) return li_launch_tc<T, 64>(p, st);
-  if (p.M <= 128) return li_launch_tc<T, 128>(p, st);
-  return li_launch_tc<T, 256>(p, st);
+  const LiForm f = li_choose(p.M, p.N, p.K);
+  if (f.pair) return li_launch_pair<T>(p, st);
+  if (f.tile == 16) return li_launch_tc<T, 16>(p, f.ksplit, st);
+  if (f.tile == 32) return li_launch_tc<T, 32>(p, f.ksplit, st);
+  if (f.tile == 64) return li_launch_tc<T, 64>(p, f.ksplit, st);
+  return li_launch_tc<T, 128>(p, f.ksplit, st);
+}
+
+static int li_read_sms() {
+  int dev = 0;
+  if (g_li_sms == 0 && (cudaGetDevice(&dev) != cudaSuccess ||
+                        cudaDeviceGetAttribute(&g_li_sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess))
+    g_li_sms = 0;
+  return g_li_sms;
+}
+
+// The kernel that a product of these sizes takes: 1000 * blocks that share a tile + tokens of a tile, negative for pairs of blocks.
+extern "C" int ullm_linear_int8_form(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0 || li_read_sms() <= 0) return 0;
+  const LiForm f = li_choose(M, N, K);
+  return f.pair ? -f.tile : 1000 * f.ksplit + f.tile;
 }
 
 // dtype: of out and bias.  Strides in bytes, at least K.
@@ -352,12 +676,7 @@ extern "C" int ullm_linear_int8(int dtype, const void* x, long long x_stride, co
   if (M < 0 || N <= 0 || N > (1 << 30) || K <= 0 || K > LI_MAX_K || x_stride < K || w_stride < K) return ULLM_ERR_BAD_SIZE;
   if (dtype != ULLM_DTYPE_F32 && dtype != ULLM_DTYPE_BF16 && dtype != ULLM_DTYPE_F16) return ULLM_ERR_BAD_DTYPE;
   if (M == 0) return ULLM_OK;
-  if (g_li_sms == 0) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&g_li_sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || g_li_sms <= 0)
-      return ULLM_ERR_LAUNCH;
-  }
+  if (li_read_sms() <= 0) return ULLM_ERR_LAUNCH;
   LiParams p = {};
   p.x = (const signed char*)x, p.w = (const signed char*)w, p.x_stride = x_stride, p.w_stride = w_stride;
   p.x_scales = (const float*)x_scales, p.w_scales = (const float*)w_scales, p.bias = bias, p.out = out;
