@@ -7,6 +7,7 @@
 //   ptr       a tensor's address (None: None)
 //   stream    the current stream's handle
 //   need      a tensor's device, type and layout; what does not hold goes on to the Python check, which says what is wrong
+//   rows      the elements between a matrix's rows, -1 where the tensor is not what a kernel takes there; vector: the same of a vector
 //   mm        out = x . w^T in bfloat16 by the vendor library, called as `torch.mm` calls it (the same handle, workspace, stream,
 //             algorithm and math mode), without the dispatcher's 4 us; False for what only `torch.mm` should decide
 //
@@ -299,6 +300,34 @@ PyObject* need(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject* kwnames
   return thrown();
 }
 
+// rows(tensor, dtype, rows, cols): the elements between the rows of a [rows, cols] matrix of that type on the current device whose columns
+// lie side by side and whose rows do not overlap (one row: as if it were padded to 16); -1 where it is none
+PyObject* rows(PyObject*, PyObject* const* args, Py_ssize_t n) try {
+  if (n != 4 || !THPVariable_Check(args[0]) || !THPDtype_Check(args[1])) return PyLong_FromLong(-1);
+  const at::Tensor& t = THPVariable_Unpack(args[0]);
+  const long long r = PyLong_AsLongLong(args[2]), c = PyLong_AsLongLong(args[3]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!t.is_cuda() || t.layout() != at::kStrided || t.scalar_type() != reinterpret_cast<THPDtype*>(args[1])->scalar_type || t.dim() != 2 ||
+      t.size(0) != r || t.size(1) != c || (c > 1 && t.stride(1) != 1) || (r > 1 && t.stride(0) < c) ||
+      t.get_device() != at::cuda::current_device())
+    return PyLong_FromLong(-1);
+  return PyLong_FromLongLong(r > 1 ? t.stride(0) : (c + 15) / 16 * 16);
+} catch (...) {
+  return thrown();
+}
+
+// vector(tensor, dtype, n): whether it holds n numbers of that type side by side, on the current device
+PyObject* vector(PyObject*, PyObject* const* args, Py_ssize_t n) try {
+  if (n != 3 || !THPVariable_Check(args[0]) || !THPDtype_Check(args[1])) Py_RETURN_FALSE;
+  const at::Tensor& t = THPVariable_Unpack(args[0]);
+  const long long size = PyLong_AsLongLong(args[2]);
+  if (PyErr_Occurred()) return nullptr;
+  return PyBool_FromLong(t.is_cuda() && t.layout() == at::kStrided && t.scalar_type() == reinterpret_cast<THPDtype*>(args[1])->scalar_type &&
+                         t.dim() == 1 && t.size(0) == size && t.is_contiguous() && t.get_device() == at::cuda::current_device());
+} catch (...) {
+  return thrown();
+}
+
 // out [M, N] (bfloat16, or float32 where `wide`) = x [M, K] . w [N, K]^T, on the current stream; the library's status
 int product(void* x, void* w, void* out, int M, int N, int K, int wide) {
   const float one = 1.f, zero = 0.f;
@@ -508,6 +537,8 @@ PyMethodDef methods[] = {
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(bind)), METH_FASTCALL, "the Launcher of a function's name and address"},
     {"ptr", ptr, METH_O, "a tensor's address"},
     {"need", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(need)), METH_FASTCALL | METH_KEYWORDS, "checks a tensor"},
+    {"rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(rows)), METH_FASTCALL, "the elements between a matrix's rows, or -1"},
+    {"vector", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(vector)), METH_FASTCALL, "whether a tensor is such a vector"},
     {"stream", stream, METH_NOARGS, "the current stream's handle on the current device"},
     {"set_slow_need", set_slow_need, METH_O, "the check that `need` falls back to"},
     {"mm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(mm)), METH_FASTCALL, "a bfloat16 product by the vendor library"},

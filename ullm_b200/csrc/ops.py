@@ -63,24 +63,36 @@ def _checked(t: torch.Tensor, name: str, dtype=None, contiguous: bool = True) ->
         raise KernelError(f"{name} must be contiguous")
 
 
-def _row_stride(t: torch.Tensor, name: str) -> int:
-    """Elements between the rows of a matrix whose columns lie side by side (a matrix of one row: as if it were padded to 16)."""
-    rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
-        raise KernelError(f"{name}: the elements of a row must lie side by side (strides {t.stride()})")
-    stride = t.stride(0)
-    if rows <= 1:
-        return -(-cols // 16) * 16
-    if stride < cols:
-        raise KernelError(f"{name}: rows overlap (strides {t.stride()}, {cols} columns)")
-    return stride
+def _here(t: torch.Tensor) -> bool:
+    return t.is_cuda and t.get_device() == torch.cuda.current_device()
 
 
-def _on_current_device(what: str, *tensors) -> None:
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != here:
-            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{here}")
+def _rows(t: torch.Tensor, dtype, rows: int, cols: int) -> int:
+    """The elements between the rows of a [rows, cols] matrix of that type on the current device whose columns lie side by side and
+    whose rows do not overlap (one row: as if it were padded to 16); -1 where it is none."""
+    if not _here(t) or t.dtype != dtype or t.shape != (rows, cols) or (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+        return -1
+    return t.stride(0) if rows > 1 else -(-cols // 16) * 16
+
+
+def _vector(t: torch.Tensor, dtype, n: int) -> bool:
+    return _here(t) and t.dtype == dtype and t.shape == (n,) and t.is_contiguous()
+
+
+def _refused(what: str, **tensors) -> None:
+    """Raises with what the tensors are, for a call that takes none like them."""
+    here = torch.cuda.current_device() if torch.cuda.is_available() else None
+    said = []
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda and here is not None:
+            raise KernelError(f"{what}: {name} is on {t.device}: the kernels run on CUDA tensors only (no CPU path)")
+        if t.is_cuda and t.get_device() != here:
+            raise KernelError(f"{what}: {name} is on {t.device}, the current device is cuda:{here}")
+        said.append(f"{name} {tuple(t.shape)} {str(t.dtype).replace('torch.', '')}"
+                    + ("" if t.is_contiguous() else f" with strides {t.stride()}"))
+    raise KernelError(f"{what}: these do not fit one another, or are of a type or layout that it does not take: " + ", ".join(said))
 
 
 # the native forms (native_call.cpp), set when the library is loaded
@@ -155,11 +167,12 @@ class _Library:
     """The compiled library: its launchers and queries as calls of native_call.cpp, any other function through ctypes."""
 
     def __init__(self, path: str):
-        global _ptr, _need, _stream, _native
+        global _ptr, _need, _stream, _native, _rows, _vector
         self._dll = ctypes.CDLL(path)
         _native = calls()
         _native.set_slow_need(_checked)
         _ptr, _need, _stream = _native.ptr, _native.need, _native.stream
+        _rows, _vector = _native.rows or _rows, _native.vector or _vector
         for name in (*LAUNCHERS, *QUERIES):
             setattr(self, name, _native.bind(name, ctypes.cast(getattr(self._dll, name), c_void_p).value))
 
@@ -795,93 +808,72 @@ class Kernels:
         """Room for 8-bit rows on borders of 16 bytes: int8 [rows, cols], contiguous where cols is a multiple of 16."""
         return torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device=device)[:, :cols]
 
-    @staticmethod
-    def _int8_out(what: str, x, rows: int, cols: int, out, scales) -> int:
-        if x.dtype not in _DT:
-            raise KernelError(f"{what}: rows of {x.dtype} (float32, bfloat16 or float16)")
-        _need(out, "out", torch.int8, False)
-        _need(scales, "scales", torch.float32)
-        if out.shape != (rows, cols) or scales.shape != (rows,) or cols < 1:
-            raise KernelError(f"{what}: {rows} rows of {cols}, out {tuple(out.shape)}, scales {tuple(scales.shape)}")
-        return _row_stride(out, f"{what}: out")
-
     @_timed("quantize_rows_int8")
     def quantize_rows_int8(self, x, out, scales):
         """out (int8 [T, C]), scales (float32 [T]) <- the rows of x [T, C] in 8 bits.  Rows of x may lie apart (a column range of wider
         ones).  A weight [N, K] is held the same way: one row and one scale per output channel."""
-        _need(x, "x", None, False)
-        if x.dim() != 2:
-            raise KernelError(f"quantize_rows_int8: x has shape {tuple(x.shape)}")
-        rows, cols = x.shape
-        stride = self._int8_out("quantize_rows_int8", x, rows, cols, out, scales)
-        _on_current_device("quantize_rows_int8", x, out, scales)
-        self._check(self.lib.ullm_quantize_rows_int8(_DT[x.dtype], _ptr(x), _row_stride(x, "quantize_rows_int8: x"), _ptr(out), stride,
-                                                     _ptr(scales), rows, cols, _stream()), f"quantize_rows_int8 (row length {cols})")
-        return out
+        if x.dim() == 2 and x.dtype in _DT:
+            rows, cols = x.shape
+            x_stride, stride = _rows(x, x.dtype, rows, cols), _rows(out, torch.int8, rows, cols)
+            if x_stride > 0 and stride > 0 and _vector(scales, torch.float32, rows):
+                code = self.lib.ullm_quantize_rows_int8(_DT[x.dtype], _ptr(x), x_stride, _ptr(out), stride, _ptr(scales), rows, cols,
+                                                        _ptr(self.status), _stream())
+                self.launches += 1
+                return out if code == 0 else self._check(code, f"quantize_rows_int8 (row length {cols})")
+        _refused("quantize_rows_int8", x=x, out=out, scales=scales)
 
     @_timed("add_rmsnorm_int8")
     def add_rmsnorm_int8(self, x, residual, weight, eps: float, out, scales):
         """`add_rmsnorm` with its result in 8 bits: s = x + residual in 32-bit, residual <- s rounded (in place; residual may be None),
         out (int8 [T, C]), scales (float32 [T]) <- the rows s / sqrt(mean(s^2) + eps) * weight."""
-        _need(x, "x")
-        _need(weight, "weight", torch.float32)
-        if x.dim() != 2:
-            raise KernelError(f"add_rmsnorm_int8: x has shape {tuple(x.shape)}")
-        rows, cols = x.shape
-        if residual is not None:
-            _need(residual, "residual", x.dtype)
-            if residual.shape != x.shape:
-                raise KernelError("add_rmsnorm_int8: residual shape differs from x")
-        if weight.shape != (cols,):
-            raise KernelError(f"add_rmsnorm_int8: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
-        stride = self._int8_out("add_rmsnorm_int8", x, rows, cols, out, scales)
-        _on_current_device("add_rmsnorm_int8", x, residual, weight, out, scales)
-        self._check(self.lib.ullm_add_rmsnorm_int8(_DT[x.dtype], _ptr(x), _ptr(residual), _ptr(weight), _ptr(out), stride, _ptr(scales),
-                                                   rows, cols, float(eps), _stream()), f"add_rmsnorm_int8 (row length {cols})")
-        return out
+        dtype = x.dtype
+        if x.dim() == 2 and dtype in _DT and x.is_contiguous():
+            rows, cols = x.shape
+            stride = _rows(out, torch.int8, rows, cols)
+            if (stride > 0 and _rows(x, dtype, rows, cols) > 0 and _vector(weight, torch.float32, cols)
+                    and _vector(scales, torch.float32, rows)
+                    and (residual is None or (_rows(residual, dtype, rows, cols) > 0 and residual.is_contiguous()))):
+                code = self.lib.ullm_add_rmsnorm_int8(_DT[dtype], _ptr(x), _ptr(residual), _ptr(weight), _ptr(out), stride, _ptr(scales),
+                                                      rows, cols, float(eps), _ptr(self.status), _stream())
+                self.launches += 1
+                return out if code == 0 else self._check(code, f"add_rmsnorm_int8 (row length {cols})")
+        _refused("add_rmsnorm_int8", x=x, residual=residual, weight=weight, out=out, scales=scales)
 
     @_timed("act_mul_int8")
     def act_mul_int8(self, gate_up, out, scales, act: int = 0):
         """`act_mul` with its result in 8 bits: out (int8 [T, I]), scales (float32 [T]) <- the rows act(gate) * up of gate_up
         [T, 2 I] = [gate | up], in 32-bit up to there (act 0 silu, 1 gelu_tanh)."""
-        _need(gate_up, "gate_up")
-        if gate_up.dim() != 2 or gate_up.shape[1] % 2:
-            raise KernelError(f"act_mul_int8: gate_up {tuple(gate_up.shape)}")
-        rows, inter = gate_up.shape[0], gate_up.shape[1] // 2
-        stride = self._int8_out("act_mul_int8", gate_up, rows, inter, out, scales)
-        _on_current_device("act_mul_int8", gate_up, out, scales)
-        self._check(self.lib.ullm_act_mul_int8(_DT[gate_up.dtype], act, _ptr(gate_up), _ptr(out), stride, _ptr(scales), rows, inter,
-                                               _stream()), f"act_mul_int8 (row length {inter})")
-        return out
+        dtype = gate_up.dtype
+        if gate_up.dim() == 2 and dtype in _DT and gate_up.is_contiguous():
+            rows, wide = gate_up.shape
+            inter = wide // 2
+            stride = _rows(out, torch.int8, rows, inter)
+            if stride > 0 and wide == 2 * inter and _rows(gate_up, dtype, rows, wide) > 0 and _vector(scales, torch.float32, rows):
+                code = self.lib.ullm_act_mul_int8(_DT[dtype], act, _ptr(gate_up), _ptr(out), stride, _ptr(scales), rows, inter,
+                                                  _ptr(self.status), _stream())
+                self.launches += 1
+                return out if code == 0 else self._check(code, f"act_mul_int8 (row length {inter}, act {act})")
+        _refused("act_mul_int8", gate_up=gate_up, out=out, scales=scales)
 
-    @_timed("linear_int8", lambda self, x, x_scales, weight, *r, **k: weight.numel())
+    @_timed("linear_int8", lambda x, x_scales, weight, *r: weight.numel())
     def linear_int8(self, x, x_scales, weight, w_scales, out, bias=None):
         """out[t, n] = (sum_k x[t, k] weight[n, k]) * x_scales[t] * w_scales[n] (+ bias[n]): x int8 [T, K], weight int8 [N, K], scales
         float32 [T] and [N], out [T, N] float32, bfloat16 or float16, bias [N] of out's type.  The sums are whole numbers and exact
         (K up to 131,071), the result is formed in 32-bit and rounded once (csrc/linear_int8.cu)."""
-        _need(x, "x", torch.int8, False)
-        _need(weight, "weight", torch.int8, False)
-        _need(x_scales, "x_scales", torch.float32)
-        _need(w_scales, "w_scales", torch.float32)
-        _need(out, "out")
-        if x.dim() != 2 or weight.dim() != 2:
-            raise KernelError(f"linear_int8: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
-        (rows, k), cols = x.shape, weight.shape[0]
-        if (weight.shape[1] != k or out.shape != (rows, cols) or x_scales.shape != (rows,) or w_scales.shape != (cols,) or cols < 1
-                or out.dtype not in _DT):
-            raise KernelError(f"linear_int8: x {tuple(x.shape)}, weight {tuple(weight.shape)}, out {tuple(out.shape)} {out.dtype}, scales "
-                              f"{tuple(x_scales.shape)} and {tuple(w_scales.shape)}")
-        if not 1 <= k <= 131071:
-            raise KernelError(f"linear_int8: k={k} (1 to 131,071: the sums are held in 32 bits)")
-        if bias is not None:
-            _need(bias, "bias", out.dtype)
-            if bias.shape != (cols,):
-                raise KernelError(f"linear_int8: bias {tuple(bias.shape)} for {cols} columns")
-        _on_current_device("linear_int8", x, x_scales, weight, w_scales, out, bias)
-        self._check(self.lib.ullm_linear_int8(_DT[out.dtype], _ptr(x), _row_stride(x, "linear_int8: x"), _ptr(x_scales), _ptr(weight),
-                                              _row_stride(weight, "linear_int8: weight"), _ptr(w_scales), _ptr(bias), _ptr(out), rows,
-                                              cols, k, _ptr(self.status), _stream()), f"linear_int8 ({rows}x{k} . {cols}x{k})")
-        return out
+        dtype = out.dtype
+        if x.dim() == 2 and weight.dim() == 2 and dtype in _DT and out.is_contiguous():
+            (rows, k), cols = x.shape, weight.shape[0]
+            x_stride, w_stride = _rows(x, torch.int8, rows, k), _rows(weight, torch.int8, cols, k)
+            if (x_stride > 0 and w_stride > 0 and cols > 0 and k <= 131071 and _rows(out, dtype, rows, cols) > 0
+                    and _vector(x_scales, torch.float32, rows) and _vector(w_scales, torch.float32, cols)
+                    and (bias is None or _vector(bias, dtype, cols))):
+                code = self.lib.ullm_linear_int8(_DT[dtype], _ptr(x), x_stride, _ptr(x_scales), _ptr(weight), w_stride, _ptr(w_scales),
+                                                 _ptr(bias), _ptr(out), rows, cols, k, _ptr(self.status), _stream())
+                self.launches += 1
+                return out if code == 0 else self._check(code, f"linear_int8 ({rows}x{k} . {cols}x{k})")
+            if k > 131071:
+                raise KernelError(f"linear_int8: k={k} (1 to 131,071: the sums are held in 32 bits)")
+        _refused("linear_int8", x=x, x_scales=x_scales, weight=weight, w_scales=w_scales, out=out, bias=bias)
 
     # -- a residual stream kept in 32-bit ---------------------------------------
     @_timed("embedding")

@@ -25,6 +25,8 @@ class PlainCalls:
     def set_slow_need(self, check) -> None:
         self.need = check
 
+    rows = vector = None  # (the Python checks of ops.py)
+
     def bind(self, name: str, address: int):
         result, types = (I, LAUNCHERS[name]) if name in LAUNCHERS else QUERIES[name]
         fn = ctypes.CFUNCTYPE(_KINDS[result])(address)

@@ -16,9 +16,13 @@
 // too).  A row that holds an infinity or a NaN has no scale: it gets the scale NaN and zeros, so that everything made of it is NaN and
 // the other rows are untouched.  (The maximum is taken of the bit patterns of |y|, in whose order infinities and then NaN come last.)
 //
-// The work is bound by memory.  A block takes a row and holds it in registers between the reduction and the store (PER groups of VEC
-// neighbouring elements per thread, all loads in flight together); rows too long for that are read a second time.
-#include "common.cuh"
+// The work is bound by memory.  Two forms:
+//   rows_int8_kernel   a block takes one row and holds it in registers between the reduction and the store (PER groups of VEC
+//                      neighbouring elements per thread, all loads in flight together); rows too long for that are read a second
+//                      time.  Few rows, and rows that do not come in pieces of 16 bytes.
+//   rows_int8_stream   blocks that stay and take one row after the other, the next rows on their way into shared memory (bulk copies)
+//                      while one is worked on.  Many rows.
+#include "tcgen05_util.cuh"
 
 #define RQ_PLAIN 0
 #define RQ_ACT 1
@@ -34,19 +38,24 @@ struct RqParams {
   int cols;
   int act;                // RQ_ACT: 0 silu, 1 gelu_tanh
   float eps;
+  int rows, depth;        // (rows_int8_stream) rows in all, rows on their way
+  int* status;
 };
 
 // a gate's activation without a branch: g / (1 + e^-z).  The fast quotient is 0 for a denominator beyond 2^126, where the true value is
-// below 2^-119.
+// below 2^-119.  The fast exponential is off by 2 + 1.16 |z| steps, less than what z's own rounding makes of it below a step; gelu's z
+// has more of that, and takes the exact one.
 __device__ __forceinline__ float rq_gate(float g, int act) {
-  const float z = act == 0 ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
-  return __fdividef(g, 1.f + expf(-z));
+  if (act == 0) return __fdividef(g, 1.f + __expf(-g));
+  return __fdividef(g, 1.f + expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));
 }
 
 // (sum, largest bit pattern) over the block, the same in every thread; the order of additions depends on blockDim alone
-__device__ __forceinline__ void rq_reduce(float& sum, uint32_t& top, bool with_sum) {
-  __shared__ float sums[32];
-  __shared__ uint32_t tops[32];
+__device__ __forceinline__ void rq_reduce(float& sum, uint32_t& top, bool with_sum, int turn = 0) {
+  __shared__ float sums_of[2][32];  // (two sets: one barrier a row)
+  __shared__ uint32_t tops_of[2][32];
+  float* sums = sums_of[turn];
+  uint32_t* tops = tops_of[turn];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   top = __reduce_max_sync(0xffffffffu, top);
   if (with_sum) sum = warp_sum(sum);
@@ -58,21 +67,19 @@ __device__ __forceinline__ void rq_reduce(float& sum, uint32_t& top, bool with_s
 }
 
 struct RqRow {
-  float pre, mul;   // out = round(v * pre * mul)
+  float mul;        // out = round(v * mul)
   uint32_t keep;    // all ones, or 0 for a row that is not finite
+  bool tiny;        // ... of v * 2^100
   float scale;
 };
 __device__ __forceinline__ RqRow rq_row(uint32_t top, float rstd) {
   RqRow r;
   const float most = __uint_as_float(top);
-  r.pre = most < 8.077935669463161e-28f ? 1.2676506002282294e30f : 1.f;  // 2^-90, 2^100
-  r.mul = top == 0u ? 0.f : 127.f / (most * r.pre);
+  r.tiny = most < 8.077935669463161e-28f;  // 2^-90
+  r.mul = top == 0u ? 0.f : 127.f / (r.tiny ? most * 1.2676506002282294e30f : most);
   r.keep = top < 0x7f800000u ? 0xffffffffu : 0u;
   r.scale = r.keep ? rstd * most / 127.f : __uint_as_float(0x7fc00000u);
   return r;
-}
-__device__ __forceinline__ uint32_t rq_round(const RqRow& r, float v) {
-  return __float_as_uint(fmaf(v * r.pre, r.mul, 12582912.f)) & r.keep;
 }
 
 // VEC values of one place of a row; RQ_NORM: unrounded sums in s beside v = s * w
@@ -109,20 +116,25 @@ __device__ __forceinline__ void rq_account(const float (&v)[VEC], const float (&
 template <int VEC>
 __device__ __forceinline__ void rq_store(const RqRow& r, signed char* out, const float (&v)[VEC]) {
   uint32_t q[VEC];
+  if (r.tiny) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) q[i] = rq_round(r, v[i]);
+    for (int i = 0; i < VEC; ++i) q[i] = __float_as_uint(fmaf(v[i] * 1.2676506002282294e30f, r.mul, 12582912.f));
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) q[i] = __float_as_uint(fmaf(v[i], r.mul, 12582912.f));
+  }
   if constexpr (VEC % 4 == 0) {
     uint32_t w[VEC / 4];
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i)
-      w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410);
+      w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410) & r.keep;
     if constexpr (VEC == 8)
       *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
     else
       *reinterpret_cast<uint32_t*>(out) = w[0];
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) out[i] = (signed char)(q[i] & 0xff);
+    for (int i = 0; i < VEC; ++i) out[i] = (signed char)(q[i] & r.keep & 0xff);
   }
 }
 
@@ -180,6 +192,122 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
   }
 }
 
+// One row after the other.  A slot of the ring holds a row's inputs one behind the other: x (RQ_ACT: gate, up), then the residual.  All of a
+// block's threads have read a slot when they meet in the reduction, so the copy of a later row into it is asked for right behind it.
+// Waits are bounded: one that runs out is recorded, and the block goes on without waiting (its rows are then wrong, and the status word
+// says so).
+template <typename T, int KIND>
+__global__ void __launch_bounds__(1024) rows_int8_stream(const RqParams p) {
+  constexpr int VEC = 16 / (int)sizeof(T), PER = 4;
+  extern __shared__ __align__(128) unsigned char rq_ring[];
+  __shared__ __align__(8) uint64_t full_bar[4];
+  const uint32_t x_bytes = (uint32_t)p.cols * (KIND == RQ_ACT ? 2 : 1) * sizeof(T);
+  const uint32_t r_bytes = KIND == RQ_NORM && p.residual != nullptr ? (uint32_t)p.cols * sizeof(T) : 0u;
+  const uint32_t slot_bytes = (x_bytes + r_bytes + 127) & ~127u;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.depth; ++s) mbar_init(&full_bar[s], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  pdl_launch_dependents();
+  __syncthreads();
+  pdl_wait();
+  auto ask = [&](long long row, int slot) {
+    const uint32_t dst = lin_smem(rq_ring + (size_t)slot * slot_bytes), bar = lin_smem(&full_bar[slot]);
+    const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_stride;
+    mbar_expect_tx(&full_bar[slot], x_bytes + r_bytes);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(x), "r"(x_bytes),
+                 "r"(bar)
+                 : "memory");
+    if (r_bytes != 0) {
+      const T* res = reinterpret_cast<const T*>(p.residual) + row * p.cols;
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + x_bytes),
+                   "l"(res), "r"(r_bytes), "r"(bar)
+                   : "memory");
+    }
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.depth; ++s)
+      if (blockIdx.x + (long long)s * gridDim.x < p.rows) ask(blockIdx.x + (long long)s * gridDim.x, s);
+  }
+  int slot = 0, turn = 0;
+  uint32_t parity = 0;
+  bool ok = true;
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    if (ok && !mbar_wait(&full_bar[slot], parity)) {
+      ullm_report(p.status, ULLM_STATUS_TIMEOUT, 138, (int)row);
+      ok = false;
+    }
+    const T* x = reinterpret_cast<const T*>(rq_ring + (size_t)slot * slot_bytes);
+    const T* res = r_bytes != 0 ? x + p.cols : nullptr;
+    float v[PER][VEC], s[VEC];
+    float sum = 0.f;
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = (i * blockDim.x + threadIdx.x) * VEC;
+      if (c < p.cols) {
+        rq_load<T, KIND, VEC>(p, x, res, c, v[i], s);
+        rq_account<KIND, VEC>(v[i], s, sum, top);
+        if (r_bytes != 0) store_vec<T, VEC>(reinterpret_cast<T*>(p.residual) + row * p.cols + c, s);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[i][e] = 0.f;
+      }
+    }
+    if (blockDim.x == 32) __syncwarp();
+    rq_reduce(sum, top, KIND == RQ_NORM, turn);
+    if (threadIdx.x == 0) {
+      const long long next = row + (long long)p.depth * gridDim.x;
+      if (ok && next < p.rows) ask(next, slot);
+    }
+    const RqRow r = rq_row(top, KIND == RQ_NORM ? rsqrtf(sum / (float)p.cols + p.eps) : 1.f);
+    if (threadIdx.x == 0) p.scales[row] = r.scale;
+    signed char* out = p.out + row * p.out_stride;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = (i * blockDim.x + threadIdx.x) * VEC;
+      if (c < p.cols) rq_store<VEC>(r, out + c, v[i]);
+    }
+    turn ^= 1;
+    if (++slot == p.depth) slot = 0, parity ^= 1;
+  }
+  if (!ok && threadIdx.x == 0)  // copies may still be on their way into the ring
+    for (int s = 0; s < p.depth; ++s) mbar_wait(&full_bar[s], s >= slot ? parity : parity ^ 1);
+}
+
+static int g_rq_sms = 0;
+
+// Many rows in pieces of 16 bytes: true where rows_int8_stream takes them (`code` is then the launch's).
+template <typename T, int KIND>
+static bool rq_launch_stream(RqParams p, int rows, cudaStream_t st, int* code) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  if (g_rq_sms == 0) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&g_rq_sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      return false;
+  }
+  const int groups = p.cols / VEC, threads = ((groups + 3) / 4 + 31) / 32 * 32;
+  const long long slot = ((long long)p.cols * sizeof(T) * (KIND == RQ_ACT || p.residual != nullptr ? 2 : 1) + 127) / 128 * 128;
+  if (rows <= 2 * g_rq_sms || p.cols < 1024 || threads > 1024 || 2 * slot > 208 * 1024) return false;
+  p.depth = slot > 12 * 1024 ? 2 : 4;
+  p.rows = rows;
+  const int smem = (int)(p.depth * slot);
+  static bool set = false;
+  if (!set) {
+    if (cudaFuncSetAttribute(rows_int8_stream<T, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024) != cudaSuccess)
+      return *code = ULLM_ERR_LAUNCH, true;
+    set = true;
+  }
+  int per_sm = 216 * 1024 / (smem + 2048);
+  if (per_sm > 1088 / threads) per_sm = 1088 / threads;  // (60 registers a thread)
+  if (per_sm > 8) per_sm = 8;
+  if (per_sm < 1) per_sm = 1;
+  const int most = per_sm * g_rq_sms, each = (rows + most - 1) / most;
+  *code = ullm_launch_kernel(rows_int8_stream<T, KIND>, dim3((rows + each - 1) / each), dim3(threads), smem, st, p);
+  return true;
+}
+
 template <typename T, int KIND, int VEC>
 static int rq_launch_vec(const RqParams& p, int rows, cudaStream_t st) {
   const int groups = (p.cols + VEC - 1) / VEC;
@@ -199,6 +327,8 @@ static int rq_launch(const RqParams& p, int rows, cudaStream_t st) {
   // 16-byte pieces of every input row, V bytes of every output row
   const bool wide = p.cols % V == 0 && (uintptr_t)p.x % 16 == 0 && p.x_stride % V == 0 && (uintptr_t)p.residual % 16 == 0 &&
                     (uintptr_t)p.weight % 16 == 0 && (uintptr_t)p.out % V == 0 && p.out_stride % V == 0;
+  int code = ULLM_OK;
+  if (wide && rq_launch_stream<T, KIND>(p, rows, st, &code)) return code;
   return wide ? rq_launch_vec<T, KIND, V>(p, rows, st) : rq_launch_vec<T, KIND, 1>(p, rows, st);
 }
 
@@ -215,24 +345,27 @@ static int rq_run(int dtype, const RqParams& p, int rows, void* stream) {
 
 // Strides in elements.
 extern "C" int ullm_quantize_rows_int8(int dtype, const void* x, long long x_stride, void* out, long long out_stride, void* scales,
-                                       int rows, int cols, void* stream) {
+                                       int rows, int cols, int* status, void* stream) {
   RqParams p = {};
+  p.status = status;
   p.x = x, p.x_stride = x_stride, p.out = (signed char*)out, p.out_stride = out_stride, p.scales = (float*)scales, p.cols = cols;
   return rq_run<RQ_PLAIN>(dtype, p, rows, stream);
 }
 
 extern "C" int ullm_act_mul_int8(int dtype, int act, const void* gate_up, void* out, long long out_stride, void* scales, int rows,
-                                 int inter, void* stream) {
+                                 int inter, int* status, void* stream) {
   if (act != 0 && act != 1) return ULLM_ERR_BAD_SIZE;
   RqParams p = {};
+  p.status = status;
   p.x = gate_up, p.x_stride = 2ll * inter, p.out = (signed char*)out, p.out_stride = out_stride, p.scales = (float*)scales;
   p.cols = inter, p.act = act;
   return rq_run<RQ_ACT>(dtype, p, rows, stream);
 }
 
 extern "C" int ullm_add_rmsnorm_int8(int dtype, const void* x, void* residual, const void* weight, void* out, long long out_stride,
-                                     void* scales, int rows, int cols, float eps, void* stream) {
+                                     void* scales, int rows, int cols, float eps, int* status, void* stream) {
   RqParams p = {};
+  p.status = status;
   p.x = x, p.x_stride = cols, p.residual = residual, p.weight = (const float*)weight, p.out = (signed char*)out;
   p.out_stride = out_stride, p.scales = (float*)scales, p.cols = cols, p.eps = eps;
   return rq_run<RQ_NORM>(dtype, p, rows, stream);
