@@ -14,7 +14,7 @@
 // bits (two's complement); |s w * (127 / max)| is at most 127 (1 + 2^-23), which is 127 again.  A row whose maximum is below 2^-90 is
 // multiplied by 2^100 first, so that 127 / max stays finite.  A row of zeros gets the scale 0 (the norm's formula: NaN where eps is 0
 // too).  A row that holds an infinity or a NaN has no scale: it gets the scale NaN and zeros, so that everything made of it is NaN and
-// the other rows are untouched.  (The maximum is taken of the bit patterns of |y|, in whose order infinities and then NaN come last.)
+// the other rows are untouched.  (Between threads the maximum is taken of bit patterns, in whose order infinities and then NaN come last.)
 //
 // The work is bound by memory.  Two forms:
 //   rows_int8_kernel   a block takes one row and holds it in registers between the reduction and the store (PER groups of VEC
@@ -38,48 +38,61 @@ struct RqParams {
   int cols;
   int act;                // RQ_ACT: 0 silu, 1 gelu_tanh
   float eps;
-  int rows, depth;        // (rows_int8_stream) rows in all, rows on their way
+  int rows;               // (rows_int8_stream)
   int* status;
 };
 
-// a gate's activation without a branch: g / (1 + e^-z).  The fast quotient is 0 for a denominator beyond 2^126, where the true value is
-// below 2^-119.  The fast exponential is off by 2 + 1.16 |z| steps, less than what z's own rounding makes of it below a step; gelu's z
-// has more of that, and takes the exact one.
+// A gate's activation g / (1 + e^-z), z = g (silu) or 2 sqrt(2 / pi) (g + 0.044715 g^3) (gelu_tanh, since (1 + tanh v) / 2 =
+// 1 / (1 + e^-2v)), in six instructions without a branch: -z log2 e, 2^x, one more, the reciprocal, two products with up's.  A
+// denominator beyond 2^126 has the reciprocal 0, where the true value is below 2^-119.  Off by 2^-22 (|z| + 2.25) of its value: a step
+// or two each, and what the roundings of the exponent make of it.
 __device__ __forceinline__ float rq_gate(float g, int act) {
-  if (act == 0) return __fdividef(g, 1.f + __expf(-g));
-  return __fdividef(g, 1.f + expf(-1.5957691216057308f * (g + 0.044715f * g * g * g)));
+  const float z = act == 0 ? g * -1.4426950408889634f : g * fmaf(g * g, -0.10294324f, -2.3022082f);
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return g * r;
+}
+// the larger magnitude, NaN where either is
+__device__ __forceinline__ float rq_max(float top, float v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(v)));
+  return r;
 }
 
-// (sum, largest bit pattern) over the block, the same in every thread; the order of additions depends on blockDim alone
-__device__ __forceinline__ void rq_reduce(float& sum, uint32_t& top, bool with_sum, int turn = 0) {
+// (sum, bits of the largest magnitude) over the block, the same in every thread; the order of additions depends on blockDim alone
+__device__ __forceinline__ uint32_t rq_reduce(float& sum, float most, bool with_sum, int turn = 0) {
   __shared__ float sums_of[2][32];  // (two sets: one barrier a row)
   __shared__ uint32_t tops_of[2][32];
   float* sums = sums_of[turn];
   uint32_t* tops = tops_of[turn];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  top = __reduce_max_sync(0xffffffffu, top);
+  uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
   if (with_sum) sum = warp_sum(sum);
-  if (warps == 1) return;
+  if (warps == 1) return top;
   if (lane == 0) tops[warp] = top, sums[warp] = sum;
   __syncthreads();
   top = __reduce_max_sync(0xffffffffu, lane < warps ? tops[lane] : 0u);
   if (with_sum) sum = warp_sum(lane < warps ? sums[lane] : 0.f);
+  return top;
 }
 
 struct RqRow {
   float mul;        // out = round(v * mul)
   uint32_t keep;    // all ones, or 0 for a row that is not finite
   bool tiny;        // ... of v * 2^100
-  float scale;
+  float most;
 };
-__device__ __forceinline__ RqRow rq_row(uint32_t top, float rstd) {
+__device__ __forceinline__ RqRow rq_row(uint32_t top) {
   RqRow r;
-  const float most = __uint_as_float(top);
+  const float most = r.most = __uint_as_float(top);
   r.tiny = most < 8.077935669463161e-28f;  // 2^-90
   r.mul = top == 0u ? 0.f : 127.f / (r.tiny ? most * 1.2676506002282294e30f : most);
   r.keep = top < 0x7f800000u ? 0xffffffffu : 0u;
-  r.scale = r.keep ? rstd * most / 127.f : __uint_as_float(0x7fc00000u);
   return r;
+}
+__device__ __forceinline__ float rq_scale(const RqRow& r, float rstd) {
+  return r.keep ? rstd * r.most / 127.f : __uint_as_float(0x7fc00000u);
 }
 
 // VEC values of one place of a row; RQ_NORM: unrounded sums in s beside v = s * w
@@ -106,10 +119,10 @@ __device__ __forceinline__ void rq_load(const RqParams& p, const T* x, const T* 
   }
 }
 template <int KIND, int VEC>
-__device__ __forceinline__ void rq_account(const float (&v)[VEC], const float (&s)[VEC], float& sum, uint32_t& top) {
+__device__ __forceinline__ void rq_account(const float (&v)[VEC], const float (&s)[VEC], float& sum, float& top) {
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    top = rq_max(top, v[i]);
     if (KIND == RQ_NORM) sum = fmaf(s[i], s[i], sum);
   }
 }
@@ -150,7 +163,7 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
   constexpr int P = PER > 0 ? PER : 1;
   float v[P][VEC], s[P][VEC];
   float sum = 0.f;
-  uint32_t top = 0u;
+  float most = 0.f;
   if constexpr (PER > 0) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -164,19 +177,18 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      rq_account<KIND, VEC>(v[i], s[i], sum, top);
+      rq_account<KIND, VEC>(v[i], s[i], sum, most);
       const int c = (i * blockDim.x + threadIdx.x) * VEC;
       if (KIND == RQ_NORM && res != nullptr && c < p.cols) store_vec<T, VEC>(res + c, s[i]);
     }
   } else {
     for (int c = threadIdx.x * VEC; c < p.cols; c += blockDim.x * VEC) {
       rq_load<T, KIND, VEC>(p, x, res, c, v[0], s[0]);
-      rq_account<KIND, VEC>(v[0], s[0], sum, top);
+      rq_account<KIND, VEC>(v[0], s[0], sum, most);
     }
   }
-  rq_reduce(sum, top, KIND == RQ_NORM);
-  const RqRow r = rq_row(top, KIND == RQ_NORM ? rsqrtf(sum / (float)p.cols + p.eps) : 1.f);
-  if (threadIdx.x == 0) p.scales[row] = r.scale;
+  const RqRow r = rq_row(rq_reduce(sum, most, KIND == RQ_NORM));
+  if (threadIdx.x == 0) p.scales[row] = rq_scale(r, KIND == RQ_NORM ? rsqrtf(sum / (float)p.cols + p.eps) : 1.f);
   if constexpr (PER > 0) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -192,20 +204,18 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
   }
 }
 
-// One row after the other.  A slot of the ring holds a row's inputs one behind the other: x (RQ_ACT: gate, up), then the residual.  All of a
-// block's threads have read a slot when they meet in the reduction, so the copy of a later row into it is asked for right behind it.
-// Waits are bounded: one that runs out is recorded, and the block goes on without waiting (its rows are then wrong, and the status word
-// says so).
+// One row after the other: two slots of shared memory hold a row's inputs each.  All of a block's threads have read a slot when they meet in
+// the reduction, so the copy of a later row into it is asked for right behind it.  Waits are bounded: one that runs out is recorded, and
+// the block goes on without waiting (its rows are then wrong, and the status word says so).
+#define RQ_SLOTS 2
 template <typename T, int KIND>
 __global__ void __launch_bounds__(1024) rows_int8_stream(const RqParams p) {
   constexpr int VEC = 16 / (int)sizeof(T), PER = 4;
   extern __shared__ __align__(128) unsigned char rq_ring[];
-  __shared__ __align__(8) uint64_t full_bar[4];
-  const uint32_t x_bytes = (uint32_t)p.cols * (KIND == RQ_ACT ? 2 : 1) * sizeof(T);
-  const uint32_t r_bytes = KIND == RQ_NORM && p.residual != nullptr ? (uint32_t)p.cols * sizeof(T) : 0u;
-  const uint32_t slot_bytes = (x_bytes + r_bytes + 127) & ~127u;
+  __shared__ __align__(8) uint64_t full_bar[RQ_SLOTS];
+  const uint32_t bytes = (uint32_t)p.cols * (KIND == RQ_ACT ? 2 : 1) * sizeof(T), slot_bytes = (bytes + 127) & ~127u;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < p.depth; ++s) mbar_init(&full_bar[s], 1);
+    for (int s = 0; s < RQ_SLOTS; ++s) mbar_init(&full_bar[s], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -213,21 +223,15 @@ __global__ void __launch_bounds__(1024) rows_int8_stream(const RqParams p) {
   __syncthreads();
   pdl_wait();
   auto ask = [&](long long row, int slot) {
-    const uint32_t dst = lin_smem(rq_ring + (size_t)slot * slot_bytes), bar = lin_smem(&full_bar[slot]);
     const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_stride;
-    mbar_expect_tx(&full_bar[slot], x_bytes + r_bytes);
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(x), "r"(x_bytes),
-                 "r"(bar)
+    mbar_expect_tx(&full_bar[slot], bytes);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     lin_smem(rq_ring + (size_t)slot * slot_bytes)),
+                 "l"(x), "r"(bytes), "r"(lin_smem(&full_bar[slot]))
                  : "memory");
-    if (r_bytes != 0) {
-      const T* res = reinterpret_cast<const T*>(p.residual) + row * p.cols;
-      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + x_bytes),
-                   "l"(res), "r"(r_bytes), "r"(bar)
-                   : "memory");
-    }
   };
   if (threadIdx.x == 0) {
-    for (int s = 0; s < p.depth; ++s)
+    for (int s = 0; s < RQ_SLOTS; ++s)
       if (blockIdx.x + (long long)s * gridDim.x < p.rows) ask(blockIdx.x + (long long)s * gridDim.x, s);
   }
   int slot = 0, turn = 0;
@@ -239,30 +243,22 @@ __global__ void __launch_bounds__(1024) rows_int8_stream(const RqParams p) {
       ok = false;
     }
     const T* x = reinterpret_cast<const T*>(rq_ring + (size_t)slot * slot_bytes);
-    const T* res = r_bytes != 0 ? x + p.cols : nullptr;
     float v[PER][VEC], s[VEC];
-    float sum = 0.f;
-    uint32_t top = 0u;
+    float sum = 0.f, most = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = (i * blockDim.x + threadIdx.x) * VEC;
       if (c < p.cols) {
-        rq_load<T, KIND, VEC>(p, x, res, c, v[i], s);
-        rq_account<KIND, VEC>(v[i], s, sum, top);
-        if (r_bytes != 0) store_vec<T, VEC>(reinterpret_cast<T*>(p.residual) + row * p.cols + c, s);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[i][e] = 0.f;
+        rq_load<T, KIND, VEC>(p, x, nullptr, c, v[i], s);
+        rq_account<KIND, VEC>(v[i], s, sum, most);
       }
     }
-    if (blockDim.x == 32) __syncwarp();
-    rq_reduce(sum, top, KIND == RQ_NORM, turn);
+    const RqRow r = rq_row(rq_reduce(sum, most, false, turn));
     if (threadIdx.x == 0) {
-      const long long next = row + (long long)p.depth * gridDim.x;
+      const long long next = row + (long long)RQ_SLOTS * gridDim.x;
       if (ok && next < p.rows) ask(next, slot);
+      p.scales[row] = rq_scale(r, 1.f);
     }
-    const RqRow r = rq_row(top, KIND == RQ_NORM ? rsqrtf(sum / (float)p.cols + p.eps) : 1.f);
-    if (threadIdx.x == 0) p.scales[row] = r.scale;
     signed char* out = p.out + row * p.out_stride;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -270,17 +266,19 @@ __global__ void __launch_bounds__(1024) rows_int8_stream(const RqParams p) {
       if (c < p.cols) rq_store<VEC>(r, out + c, v[i]);
     }
     turn ^= 1;
-    if (++slot == p.depth) slot = 0, parity ^= 1;
+    if (++slot == RQ_SLOTS) slot = 0, parity ^= 1;
   }
-  if (!ok && threadIdx.x == 0)  // copies may still be on their way into the ring
-    for (int s = 0; s < p.depth; ++s) mbar_wait(&full_bar[s], s >= slot ? parity : parity ^ 1);
+  if (!ok && threadIdx.x == 0)  // copies may still be on their way into the slots
+    for (int s = 0; s < RQ_SLOTS; ++s) mbar_wait(&full_bar[s], s >= slot ? parity : parity ^ 1);
 }
 
 static int g_rq_sms = 0;
 
-// Many rows in pieces of 16 bytes: true where rows_int8_stream takes them (`code` is then the launch's).
+// True where rows_int8_stream takes the rows (`code` is then the launch's): many and long ones.  us there and below: 2,048 x 25,600 gated
+// 53.7 and 75.7, 2,048 x 16,384 plain 18.8 and 25.9, 1,000 11.7 and 14.3, 300 6.6 and 6.1; 2,048 x 8,192 plain 11.8 and 12.2, gated 19.6
+// and 19.4.  A norm reads its weight beside the rows and is never faster there (2,048 x 4,096 14.2 and 13.0).
 template <typename T, int KIND>
-static bool rq_launch_stream(RqParams p, int rows, cudaStream_t st, int* code) {
+static bool rq_try_stream(RqParams p, int rows, cudaStream_t st, int* code) {
   constexpr int VEC = 16 / (int)sizeof(T);
   if (g_rq_sms == 0) {
     int dev = 0;
@@ -288,11 +286,9 @@ static bool rq_launch_stream(RqParams p, int rows, cudaStream_t st, int* code) {
       return false;
   }
   const int groups = p.cols / VEC, threads = ((groups + 3) / 4 + 31) / 32 * 32;
-  const long long slot = ((long long)p.cols * sizeof(T) * (KIND == RQ_ACT || p.residual != nullptr ? 2 : 1) + 127) / 128 * 128;
-  if (rows <= 2 * g_rq_sms || p.cols < 1024 || threads > 1024 || 2 * slot > 208 * 1024) return false;
-  p.depth = slot > 12 * 1024 ? 2 : 4;
-  p.rows = rows;
-  const int smem = (int)(p.depth * slot);
+  const long long slot = ((long long)p.cols * sizeof(T) * (KIND == RQ_ACT ? 2 : 1) + 127) / 128 * 128;
+  if (rows < 4 * g_rq_sms || groups < 2048 || groups > 4096 || RQ_SLOTS * slot > 208 * 1024) return false;
+  const int smem = (int)(RQ_SLOTS * slot);
   static bool set = false;
   if (!set) {
     if (cudaFuncSetAttribute(rows_int8_stream<T, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024) != cudaSuccess)
@@ -301,13 +297,16 @@ static bool rq_launch_stream(RqParams p, int rows, cudaStream_t st, int* code) {
   }
   int per_sm = 216 * 1024 / (smem + 2048);
   if (per_sm > 1088 / threads) per_sm = 1088 / threads;  // (60 registers a thread)
-  if (per_sm > 8) per_sm = 8;
   if (per_sm < 1) per_sm = 1;
-  const int most = per_sm * g_rq_sms, each = (rows + most - 1) / most;
+  const int most = per_sm * g_rq_sms, each = (rows + most - 1) / most;  // (every block the same number of rows, or one less)
+  p.rows = rows;
   *code = ullm_launch_kernel(rows_int8_stream<T, KIND>, dim3((rows + each - 1) / each), dim3(threads), smem, st, p);
   return true;
 }
 
+// Groups of a thread.  One, where a row's groups are threads enough: 2,048 x 4,096 normed 13.0 us, with two 15.2; rows as they are are
+// less work and take two from 256 groups on (2,048 x 4,096 6.7 for 8.0, 8 x 8,192 1.61 for 1.69).  Element by element many rows take two
+// from 384 on and four from 768 (1,000 x 2,043 normed 9.7, with two 11.7, with eight 13.3; 1,000 x 531 3.3, with one 4.8).
 template <typename T, int KIND, int VEC>
 static int rq_launch_vec(const RqParams& p, int rows, cudaStream_t st) {
   const int groups = (p.cols + VEC - 1) / VEC;
@@ -315,8 +314,12 @@ static int rq_launch_vec(const RqParams& p, int rows, cudaStream_t st) {
     int threads = ((groups + per - 1) / per + 31) / 32 * 32;
     return ullm_launch_kernel(kernel, dim3(rows), dim3(threads > 1024 ? 1024 : threads), 0, st, p);
   };
-  if (groups <= 1024) return go(rows_int8_kernel<T, KIND, VEC, 1>, 1);
-  if (groups <= 2048) return go(rows_int8_kernel<T, KIND, VEC, 2>, 2);
+  const int least = VEC == 1 ? (rows <= 256 || groups < 384 ? 1 : groups < 768 ? 2 : 4) : KIND == RQ_PLAIN && groups >= 256 ? 2 : 1;
+  if constexpr (VEC == 1) {
+    if (groups > 4096 && groups <= 8192) return go(rows_int8_kernel<T, KIND, VEC, 8>, 8);
+  }
+  if (groups <= 1024 && least < 2) return go(rows_int8_kernel<T, KIND, VEC, 1>, 1);
+  if (groups <= 2048 && least < 3) return go(rows_int8_kernel<T, KIND, VEC, 2>, 2);
   if (groups <= 4096) return go(rows_int8_kernel<T, KIND, VEC, 4>, 4);
   return go(rows_int8_kernel<T, KIND, VEC, 0>, 4);
 }
@@ -328,7 +331,9 @@ static int rq_launch(const RqParams& p, int rows, cudaStream_t st) {
   const bool wide = p.cols % V == 0 && (uintptr_t)p.x % 16 == 0 && p.x_stride % V == 0 && (uintptr_t)p.residual % 16 == 0 &&
                     (uintptr_t)p.weight % 16 == 0 && (uintptr_t)p.out % V == 0 && p.out_stride % V == 0;
   int code = ULLM_OK;
-  if (wide && rq_launch_stream<T, KIND>(p, rows, st, &code)) return code;
+  if constexpr (KIND != RQ_NORM) {
+    if (wide && rq_try_stream<T, KIND>(p, rows, st, &code)) return code;
+  }
   return wide ? rq_launch_vec<T, KIND, V>(p, rows, st) : rq_launch_vec<T, KIND, 1>(p, rows, st);
 }
 
