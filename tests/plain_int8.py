@@ -48,3 +48,27 @@ def check_product(got, ref, size):
     limit = size * 2 * 2.0 ** -24 * 1.01 + ref.abs() * (2.0 ** -24 + (HALF[dt] if dt != torch.float32 else 0.0)) * 1.01 + TINY[dt]
     err = (got.double() - ref).abs()
     assert (err <= limit).all(), f"{int((err > limit).sum())} of {err.numel()} results off, up to {float((err / limit).max()):.2f} of the limit"
+
+
+class HeldMatrix:
+    """A weight in 8 bits as the plain model's products meet it: h @ W.T with W's rows and h's as the values that they are held as."""
+
+    def __init__(self, w):
+        self.held = held(w)
+
+    @property
+    def T(self):
+        return self
+
+    def __rmatmul__(self, h):
+        return held(h) @ self.held.T
+
+
+def held(y):
+    step = y.abs().amax(-1, keepdim=True) / 127
+    return torch.where(step > 0, torch.round(y / step) * step, 0.0)
+
+
+def held_weights(w):
+    """The plain model's weights with the layers' matrices in 8 bits."""
+    return {n: HeldMatrix(t.double()) if n.endswith("_proj.weight") else t.double() for n, t in w.items()}

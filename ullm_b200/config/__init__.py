@@ -1,5 +1,6 @@
 from .borosun import BorosunConfig, BorosunConfigError, borosun_model_spec
 from .engine_config import EngineConfig
+from .int8 import QUANTIZATIONS, int8_spec
 from .finosun import FinosunConfig, FinosunConfigError, finosun_model_spec
 from .mafarax import MafaraxConfig, MafaraxConfigError, mafarax_model_spec
 from .pidenex import PidenexConfig, PidenexConfigError, pidenex_model_spec
@@ -35,7 +36,7 @@ register_architecture("Mafarax", MafaraxConfig.from_dict, mafarax_model_spec)
 register_architecture("Ninelix", NinelixConfig.from_dict, ninelix_model_spec, reads_shapes=True)
 
 __all__ = [
-    "ARCHITECTURES", "Architecture", "BorosunConfig", "BorosunConfigError", "borosun_model_spec", "ConfigError", "EngineConfig", "FeedForwardSpec", "FinosunConfig", "FinosunConfigError", "finosun_model_spec", "LayerSpec",
+    "ARCHITECTURES", "Architecture", "BorosunConfig", "BorosunConfigError", "borosun_model_spec", "ConfigError", "EngineConfig", "FeedForwardSpec", "QUANTIZATIONS", "int8_spec", "FinosunConfig", "FinosunConfigError", "finosun_model_spec", "LayerSpec",
     "LudalixConfig", "LudalixConfigError", "ludalix_model_spec", "MafaraxConfig", "MafaraxConfigError", "mafarax_model_spec", "NinelixConfig", "NinelixConfigError", "ninelix_model_spec", "PairEmbeddingSpec", "PidenexConfig", "PidenexConfigError", "pidenex_model_spec", "MixerSpec", "ModelSpec", "NormSpec", "PositionSpec", "Qwen3Config", "ScheduleEntry", "TokenSideSpec",
     "load_model_spec", "qwen3_model_spec", "read_config_json", "register_architecture",
     "resolve_architecture",

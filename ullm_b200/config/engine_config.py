@@ -44,6 +44,7 @@ class EngineConfig:
     num_pages: int | None = None  # None: sized from free memory x gpu_memory_utilization
     enable_prefix_caching: bool = True
     warmup_graphs: bool = False  # record every decode graph while the engine starts instead of at first use
+    quantization: str | None = None  # "int8": the layers' products in 8-bit integers (pre-norm decoders; parts/int8.py)
     random_init_std: float = 0.02
     random_init_norm_std: float = 0.0
 
@@ -68,8 +69,11 @@ class EngineConfig:
                 raise ValueError(f"Unsupported dtype {self.dtype!r} (bfloat16, float16 or float32)")
         if self.load_format not in ("safetensors", "random"):
             raise ValueError("load_format is 'safetensors' or 'random'")
+        from .int8 import QUANTIZATIONS
         from .registry import read_config_json
 
+        if self.quantization is not None and self.quantization not in QUANTIZATIONS:
+            raise ValueError(f"quantization is None or one of {QUANTIZATIONS}, not {self.quantization!r}")
         self.model_config = read_config_json(self.model)
         gpath = os.path.join(self.model, "generation_config.json")
         self.generation_config = None
@@ -114,6 +118,7 @@ class EngineConfig:
         parser.add_argument("--max-num-batched-tokens", type=int, default=2048, help="Token budget of one step")
         parser.add_argument("--dtype", type=str, default=None, help="bfloat16, float16 or float32 (default: config.json's; the fast attention kernels are bfloat16)")
         parser.add_argument("--load-format", type=str, default="safetensors", help="safetensors or random")
+        parser.add_argument("--quantization", type=str, default=None, help="int8: the layers' products in 8-bit integers, with a scale per token and per output channel")
         parser.add_argument("--seed", type=int, default=0, help="Seed of random weights and of sampling")
         parser.add_argument("--num-pages", type=int, default=None, help="KV pages (default: from free memory)")
         parser.add_argument("--no-prefix-caching", action="store_true", help="Disable prefix reuse over pages")
@@ -142,6 +147,7 @@ class EngineConfig:
             dtype=getattr(args, "dtype", None),
             load_format=getattr(args, "load_format", "safetensors"),
             seed=getattr(args, "seed", 0),
+            quantization=getattr(args, "quantization", None),
             num_pages=getattr(args, "num_pages", None),
             enable_prefix_caching=not getattr(args, "no_prefix_caching", False),
             warmup_graphs=getattr(args, "warmup_graphs", False),

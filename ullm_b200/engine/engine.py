@@ -40,6 +40,7 @@ class Engine:
             random_std=config.random_init_std,
             random_norm_std=config.random_init_norm_std,
             enable_prefix_cache=config.enable_prefix_caching,
+            quantization=config.quantization,
         )
         cache = self.runner.cache
         logger.info("model ready in %.1f s; KV cache: %d pages of %d tokens (%d tokens)", time.time() - t0,

@@ -19,6 +19,7 @@ import numpy as np
 import torch
 
 from ..cache import CacheManager, OutOfPages, RequestCache
+from ..config.int8 import QUANTIZATIONS, int8_spec
 from ..config.registry import load_model_spec
 from ..csrc import kernels
 from ..parts.model import DecoderModel
@@ -63,11 +64,16 @@ class ModelRunner:
         enable_prefix_cache: bool = False,
         poison_cache: bool = False,
         progress=None,
+        quantization: str | None = None,
     ):
         if model_dir is None and config is None:
             raise ValueError("a model folder or a config dict is needed")
         self.device = torch.device(device)
         self.typed_config, self.spec = load_model_spec(config if config is not None else model_dir)
+        if quantization is not None:
+            if quantization not in QUANTIZATIONS:
+                raise ValueError(f"quantization is None or one of {QUANTIZATIONS}, not {quantization!r}")
+            self.spec = int8_spec(self.spec)
         self.dtype = engine_dtype(dtype, self.spec.dtype)
         self.checkpoint_dtype = self.spec.dtype
         if self.dtype == torch.float16:
@@ -93,6 +99,8 @@ class ModelRunner:
             fill_random_(self.model, seed, random_std, random_norm_std)
         else:
             raise ValueError(f"unknown load_format {load_format!r}")
+        if quantization is not None and self.device.type == "cuda":
+            torch.cuda.empty_cache()  # (the matrices as they came, which the 8-bit ones have replaced)
 
         self.page_size = page_size
         self.max_context = min(max_context, self.spec.max_positions)
