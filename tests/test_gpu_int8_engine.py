@@ -8,6 +8,7 @@ import plain_model as pm
 from helpers import errors, plain_logits, random_ids, weights_for, write_model_dir
 from plain_int8 import held_weights
 from test_gpu_replay import run_cut
+from ullm_b200.csrc import kernels
 
 pytestmark = [pytest.mark.gpu, pytest.mark.needs_cuda]
 
@@ -96,3 +97,34 @@ def test_random_weights_on_the_device(tmp_path):
         # 8 bits beside 8 bits of mantissa: a step of noise of 1 / 254 of the largest against 2^-9 of each element
         assert torch.isfinite(b).all() and (a - b).abs().max() <= 0.1 * a.abs().max()
         assert not torch.equal(a, b)
+
+
+def test_prompts_one_after_another(tmp_path):
+    """Many prompt steps in a row, so that every kernel may begin beside the end of the one in front of it: each as when it runs alone.
+    (Products by pairs of SMs allocate tensor memory for both: a block that did so before the other one had started waited for good.)"""
+    from ullm_b200.engine import ModelRunner, StepEntry
+
+    cfg = dict(architectures=["Qwen3ForCausalLM"], num_hidden_layers=6, hidden_size=2048, num_attention_heads=16, num_key_value_heads=4,
+               head_dim=128, intermediate_size=8192, vocab_size=1000, rope_theta=1e6, rms_norm_eps=1e-6, attention_bias=False,
+               tie_word_embeddings=False, max_position_embeddings=4096, torch_dtype="bfloat16")
+    r = ModelRunner(config=cfg, page_size=16, num_pages=260, max_requests=2, max_context=4096, max_step_tokens=2048,
+                    load_format="random", seed=3, quantization="int8")
+    ids = random_ids(1000, 2000, 4)
+    assert kernels().lib.ullm_linear_int8_form(2000, 2 * 8192, 2048) < 0
+
+    def prompt(n):
+        r.add_request("a")
+        out = r.step([StepEntry("a", ids[:n], [n - 1])]).clone()
+        r.end_request("a")
+        return out
+
+    sizes = (2000, 700, 1024)
+    alone = []
+    for n in sizes:
+        alone.append(prompt(n))
+        torch.cuda.synchronize()
+    for _ in range(30):
+        got = [prompt(n) for n in sizes]
+    for a, b in zip(alone, got):
+        assert torch.equal(a, b)
+    r.check_device_status()

@@ -404,6 +404,10 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  __syncthreads();
+  li_cluster_sync();  // the other block runs and its barriers exist
+  // Allocating for a pair takes both blocks: what one asks of the other's SM is lost for good where that block has not started yet, or
+  // has ended.  So it stands behind the cluster's first meeting, and giving back in front of its last one.
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lin_smem(&tmem_slot)), "r"(2 * BN)
                  : "memory");
@@ -412,7 +416,6 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  li_cluster_sync();  // the other block's barriers exist
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_d = tmem_slot;
   pdl_wait();
@@ -437,6 +440,14 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
           li_pair_load(st + LI_W_BYTES, &x_map, bar, kb * 128, t0);
           if (++s == LI_PAIR_STAGES) s = 0, parity ^= 1;
         }
+      }
+      // (the commits that free the last stages arrive in both blocks: neither ends before)
+      for (int i = 0; i < LI_PAIR_STAGES && ok; ++i) {
+        if (!mbar_wait(&empty_bar[s], parity)) {
+          ullm_report(p.status, ULLM_STATUS_TIMEOUT, 139, i);
+          ok = false;
+        }
+        if (++s == LI_PAIR_STAGES) s = 0, parity ^= 1;
       }
     }
     __syncwarp();
@@ -518,6 +529,7 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_d), "r"(2 * BN) : "memory");
   }
+  li_cluster_sync();  // (see the allocation)
 }
 
 // rows of 8-bit numbers, boxes of box_rows x 128 bytes
