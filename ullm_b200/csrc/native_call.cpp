@@ -308,7 +308,7 @@ PyObject* rows(PyObject*, PyObject* const* args, Py_ssize_t n) try {
   const long long r = PyLong_AsLongLong(args[2]), c = PyLong_AsLongLong(args[3]);
   if (PyErr_Occurred()) return nullptr;
   if (!t.is_cuda() || t.layout() != at::kStrided || t.scalar_type() != reinterpret_cast<THPDtype*>(args[1])->scalar_type || t.dim() != 2 ||
-      t.size(0) != r || t.size(1) != c || (c > 1 && t.stride(1) != 1) || (r > 1 && t.stride(0) < c) ||
+      t.size(0) != r || t.size(1) != c || r > INT_MAX || c > INT_MAX || (c > 1 && t.stride(1) != 1) || (r > 1 && t.stride(0) < c) ||
       t.get_device() != at::cuda::current_device())
     return PyLong_FromLong(-1);
   return PyLong_FromLongLong(r > 1 ? t.stride(0) : (c + 15) / 16 * 16);

@@ -70,7 +70,7 @@ def _here(t: torch.Tensor) -> bool:
 def _rows(t: torch.Tensor, dtype, rows: int, cols: int) -> int:
     """The elements between the rows of a [rows, cols] matrix of that type on the current device whose columns lie side by side and
     whose rows do not overlap (one row: as if it were padded to 16); -1 where it is none."""
-    if not _here(t) or t.dtype != dtype or t.shape != (rows, cols) or (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+    if not _here(t) or t.dtype != dtype or t.shape != (rows, cols) or max(rows, cols) >= 1 << 31 or (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
         return -1
     return t.stride(0) if rows > 1 else -(-cols // 16) * 16
 
@@ -92,7 +92,7 @@ def _refused(what: str, **tensors) -> None:
             raise KernelError(f"{what}: {name} is on {t.device}, the current device is cuda:{here}")
         said.append(f"{name} {tuple(t.shape)} {str(t.dtype).replace('torch.', '')}"
                     + ("" if t.is_contiguous() else f" with strides {t.stride()}"))
-    raise KernelError(f"{what}: these do not fit one another, or are of a type or layout that it does not take: " + ", ".join(said))
+    raise KernelError(f"{what}: these do not fit one another, or are of a type, layout or device that it does not take: " + ", ".join(said))
 
 
 # the native forms (native_call.cpp), set when the library is loaded
@@ -187,6 +187,7 @@ class Kernels:
         self.lib_path = lib_path or build()
         self._declare(self.lib_path)
         self.status = torch.zeros(4, dtype=torch.int32, device="cuda")
+        self.device_index = self.status.get_device()
         self.sm_count = torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
         self._f32_out_mm = None
         self._moe_plain = False
@@ -357,6 +358,10 @@ class Kernels:
         self.lib = _Library(path)
         self.lib.ullm_lt_last_choice.argtypes = [c_void_p] * 4
         self.lib.ullm_lt_last_choice.restype = None
+
+    def _elsewhere(self, t) -> bool:
+        """Whether a tensor lies on another device than these kernels were set up for."""
+        return t.get_device() != self.device_index
 
     def _check(self, code: int, what: str) -> None:
         self.launches += 1
@@ -812,7 +817,7 @@ class Kernels:
     def quantize_rows_int8(self, x, out, scales):
         """out (int8 [T, C]), scales (float32 [T]) <- the rows of x [T, C] in 8 bits.  Rows of x may lie apart (a column range of wider
         ones).  A weight [N, K] is held the same way: one row and one scale per output channel."""
-        if x.dim() == 2 and x.dtype in _DT:
+        if x.dim() == 2 and x.dtype in _DT and not self._elsewhere(x):
             rows, cols = x.shape
             x_stride, stride = _rows(x, x.dtype, rows, cols), _rows(out, torch.int8, rows, cols)
             if x_stride > 0 and stride > 0 and _vector(scales, torch.float32, rows):
@@ -827,7 +832,7 @@ class Kernels:
         """`add_rmsnorm` with its result in 8 bits: s = x + residual in 32-bit, residual <- s rounded (in place; residual may be None),
         out (int8 [T, C]), scales (float32 [T]) <- the rows s / sqrt(mean(s^2) + eps) * weight."""
         dtype = x.dtype
-        if x.dim() == 2 and dtype in _DT and x.is_contiguous():
+        if x.dim() == 2 and dtype in _DT and x.is_contiguous() and not self._elsewhere(x):
             rows, cols = x.shape
             stride = _rows(out, torch.int8, rows, cols)
             if (stride > 0 and _rows(x, dtype, rows, cols) > 0 and _vector(weight, torch.float32, cols)
@@ -844,7 +849,7 @@ class Kernels:
         """`act_mul` with its result in 8 bits: out (int8 [T, I]), scales (float32 [T]) <- the rows act(gate) * up of gate_up
         [T, 2 I] = [gate | up], in 32-bit up to there (act 0 silu, 1 gelu_tanh)."""
         dtype = gate_up.dtype
-        if gate_up.dim() == 2 and dtype in _DT and gate_up.is_contiguous():
+        if gate_up.dim() == 2 and dtype in _DT and gate_up.is_contiguous() and not self._elsewhere(gate_up):
             rows, wide = gate_up.shape
             inter = wide // 2
             stride = _rows(out, torch.int8, rows, inter)
@@ -861,7 +866,7 @@ class Kernels:
         float32 [T] and [N], out [T, N] float32, bfloat16 or float16, bias [N] of out's type.  The sums are whole numbers and exact
         (K up to 131,071), the result is formed in 32-bit and rounded once (csrc/linear_int8.cu)."""
         dtype = out.dtype
-        if x.dim() == 2 and weight.dim() == 2 and dtype in _DT and out.is_contiguous():
+        if x.dim() == 2 and weight.dim() == 2 and dtype in _DT and out.is_contiguous() and not self._elsewhere(x):
             (rows, k), cols = x.shape, weight.shape[0]
             x_stride, w_stride = _rows(x, torch.int8, rows, k), _rows(weight, torch.int8, cols, k)
             if (x_stride > 0 and w_stride > 0 and cols > 0 and k <= 131071 and _rows(out, dtype, rows, cols) > 0
