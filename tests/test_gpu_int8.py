@@ -300,3 +300,52 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for ops, out in zip(sets, outs):
         check_product(out, *product(*ops))
+
+
+def test_graphs_side_by_side():
+    """Two recorded graphs of the same products, replayed on two streams at once: nothing is shared between them."""
+    kk = K()
+    sets = [operands(30 + i, 24, 2000, 8192) for i in range(2)]
+    outs = [torch.empty(24, 2000, device=device()) for _ in range(2)]
+    graphs, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    for ops, out in zip(sets, outs):
+        kk.linear_int8(*ops, out)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            for _ in range(5):
+                kk.linear_int8(*ops, out)
+    for out in outs:
+        out.fill_(9.0)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for ops, out in zip(sets, outs):
+        check_product(out, *product(*ops))
+
+
+def test_more_than_31_bits_of_elements():
+    """A weight of 2.3 G elements made and used, a result of 2.4 G: rows past the 31st bit are where they belong."""
+    kk, N, k = K(), 70001, 32768
+    w = torch.zeros(N, k, dtype=torch.bfloat16, device=device())
+    last = rows_of(gen(1), 300, k, torch.bfloat16)
+    w[-300:], w[:300] = last, last.flip(0)
+    q, s = kk.int8_rows(N, k), torch.empty(N, device=device())
+    kk.quantize_rows_int8(w, q, s)
+    del w
+    check_rows(q[-300:], s[-300:], last.double(), 0.0, 2.0 ** -24 * 1.01)
+    assert torch.equal(q[:300], q[-300:].flip(0)) and not s[300:-300].any() and not q[40000].any()
+    for M in (3, 300):
+        x, xs, _, _ = operands(2, M, 1, k)
+        out = run(x, xs, q, s, torch.bfloat16)
+        check_product(out[:, -300:], *product(x, xs, q[-300:], s[-300:]))
+        assert torch.equal(out[:, :300], out[:, -300:].flip(1)) and not out[:, 300:-300].any()
+    del q, out
+    M, N, k = 40000, 60001, 48
+    x, xs, w, ws = operands(3, M, N, k)
+    out = run(x, xs, w, ws, torch.bfloat16)
+    for rows in (slice(0, 64), slice(35000, 35064), slice(M - 64, M)):
+        check_product(out[rows], *product(x[rows], xs[rows], w, ws))

@@ -35,7 +35,8 @@ class Int8Rows:
 
     def times(self, weight: "Int8Matrix", out, bias=None):
         """out = these rows . weight^T (+ bias)"""
-        return kernels().linear_int8(self.q, self.scales, weight.q, weight.scales, out, bias)
+        kernels().linear_int8(self.q, self.scales, weight.q, weight.scales, out, bias)
+        return out
 
 
 class Int8Matrix:
