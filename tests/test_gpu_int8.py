@@ -156,7 +156,8 @@ PRODUCTS = [(1, 1, 16), (1, 6144, 4096), (2, 128, 128), (7, 130, 144), (8, 24576
             (200, 2048, 2048), (256, 640, 512), (257, 1000, 784), (511, 4096, 256), (1000, 2500, 528), (2048, 4096, 4096),
             (16, 7156, 5232), (13, 2000, 8208), (16, 6144, 2064), (20, 300, 2064), (30, 2000, 8208), (31, 6100, 2064), (31, 6683, 7072), (32, 12300, 1040),
             (61, 5000, 2064), (40, 520, 2064), (64, 10000, 528), (100, 24500, 272), (97, 4666, 4320), (125, 6100, 2064), (300, 4090, 2064),
-            (333, 12200, 1040), (120, 2393, 5856), (513, 6200, 1040), (2047, 4095, 272), (700, 20001, 400)]
+            (333, 12200, 1040), (120, 2393, 5856), (513, 6200, 1040), (2047, 4095, 272), (700, 20001, 400),
+            (6, 4239, 5808), (4, 837, 2512), (19, 1279, 5904), (75, 5209, 7872), (91, 2059, 4640), (1, 6144, 4112)]
 
 
 def test_the_products_take_every_form():

@@ -10,6 +10,8 @@
 //   linear_int8_pair    the same for many tokens, two SMs to a tile;
 //   linear_int8_plain   rows at any address, four products an instruction (dp4a).
 // `li_choose` says which of the first two takes a product.
+#include <cmath>
+
 #include "tcgen05_util.cuh"
 
 #define LI_MAX_K 131071
@@ -101,7 +103,7 @@ __global__ void __launch_bounds__(256) linear_int8_plain(const LiParams p) {
 // ---------------------------------------------------------------------------------------------
 // The tensor cores.  A tile is 128 channels by NT tokens: channels are the instruction's M (the lanes of tensor memory), tokens its N
 // (16 to 128), so that few tokens cost few columns and every weight byte still meets a full instruction.  A block of six warps:
-//   warp 0 (one lane)  TMA loads of 128 k of both operands (128-byte swizzle) into a ring of stages;
+//   warp 0             TMA loads of both operands (128-byte swizzle) into a ring of stages, KB blocks of 128 k each;
 //   warp 1             tcgen05.mma, 32 k an instruction, the accumulator (32-bit whole numbers) in tensor memory;
 //   warps 2 to 5       the end: a thread owns a channel; a warp stores 32 neighbouring channels of a token at a time.
 // With few tiles a cluster of `ksplit` blocks shares one, each with a range of K: every block then hands each of the others its sums of
@@ -145,15 +147,31 @@ __device__ __forceinline__ void li_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// The copies are asked for by a whole warp, one lane's predicate before the instructions: addresses then stay in uniform registers.  By one
+// lane in a branch of its own a stage of 128 k took 0.25 us to ask for, whatever its size, so 0.15.
+__device__ __forceinline__ void li_expect(uint32_t lead, uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %0, 0;\n @q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%1], %2;\n}\n"
+      ::"r"(lead), "r"(bar), "r"(bytes)
+      : "memory");
+}
+__device__ __forceinline__ void li_load(uint32_t lead, uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %0, 0;\n"
+      " @q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%1], [%2, {%4, %5}], [%3];\n}\n"
+      ::"r"(lead), "r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+
 // instruction descriptor of kind::i8: 32-bit sums, signed operands, both K-major
 __host__ __device__ constexpr uint32_t li_idesc(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-template <typename T, int NT>
+template <typename T, int NT, int KB>
 __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_constant__ CUtensorMap w_map,
                                                            const __grid_constant__ CUtensorMap x_map, const LiParams p) {
-  constexpr int STAGE = LI_W_BYTES + NT * 128;
+  constexpr int BLOCK = LI_W_BYTES + NT * 128, STAGE = KB * BLOCK;  // 128 k of both operands; a stage
   constexpr int TMEM = NT < 32 ? 32 : NT;
   extern __shared__ unsigned char li_smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[LI_MAX_STAGES], empty_bar[LI_MAX_STAGES], acc_bar;
@@ -164,8 +182,8 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)blockIdx.x % p.ksplit, n0 = (int)blockIdx.x / p.ksplit * 128;
   const int m0 = (int)blockIdx.y * NT;
-  const int kb0 = (int)((long long)p.k_blocks * rank / p.ksplit), kb1 = (int)((long long)p.k_blocks * (rank + 1) / p.ksplit);
-  const int nkb = kb1 - kb0;  // >= 1: the host splits no further than there are blocks
+  const int all = (p.k_blocks + KB - 1) / KB;  // stages of the whole k; this block's are st0 .. st0 + nst - 1, at least one
+  const int st0 = (int)((long long)all * rank / p.ksplit), nst = (int)((long long)all * (rank + 1) / p.ksplit) - st0;
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -183,7 +201,7 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     pdl_launch_dependents();  // (only now: a kernel behind this one must not hold tensor memory that this one waits for)
   }
-  if (warp == 0 && lane < p.stages && lane < nkb) li_prefetch(&w_map, (kb0 + lane) * 128, n0);
+  if (warp == 0 && lane < p.stages * KB && lane < nst * KB) li_prefetch(&w_map, (st0 * KB + lane) * 128, n0);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -192,30 +210,32 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
 
   bool ok = true;
   if (warp == 0) {
-    if (lane == 0) {
-      int s = 0;
-      uint32_t parity = 1;  // a fresh barrier passes a wait on parity 1
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&empty_bar[s], parity)) {
-          ullm_report(p.status, ULLM_STATUS_TIMEOUT, 131, kb);
-          abort_flag = 1;
-          break;
-        }
-        unsigned char* st = ring + s * STAGE;
-        mbar_expect_tx(&full_bar[s], STAGE);
-        tma_load_2d(st, &w_map, &full_bar[s], kb * 128, n0);
-        tma_load_2d(st + LI_W_BYTES, &x_map, &full_bar[s], kb * 128, m0);
-        if (++s == p.stages) s = 0, parity ^= 1;
+    const uint32_t lead = elect_one();
+    const uint32_t ring0 = lin_smem(ring), full0 = lin_smem(&full_bar[0]), empty0 = lin_smem(&empty_bar[0]);
+    int s = 0, x = st0 * KB * 128;
+    uint32_t parity = 1;  // a fresh barrier passes a wait on parity 1
+    for (int i = 0; i < nst; ++i, x += KB * 128) {
+      if (!__all_sync(0xffffffffu, mbar_wait_addr(empty0 + s * 8, parity))) {
+        if (lane == 0) ullm_report(p.status, ULLM_STATUS_TIMEOUT, 131, i);
+        abort_flag = 1;
+        break;
       }
+      const uint32_t st = ring0 + s * STAGE, bar = full0 + s * 8;
+      li_expect(lead, bar, STAGE);
+#pragma unroll
+      for (int b = 0; b < KB; ++b) {
+        li_load(lead, st + b * BLOCK, &w_map, bar, x + b * 128, n0);
+        li_load(lead, st + b * BLOCK + LI_W_BYTES, &x_map, bar, x + b * 128, m0);
+      }
+      if (++s == p.stages) s = 0, parity ^= 1;
     }
-    __syncwarp();
   } else if (warp == 1) {
     constexpr uint32_t idesc = li_idesc(128, NT);
     const uint32_t lead = elect_one();
     const uint64_t desc0 = umma_desc(ring);
     int s = 0;
     uint32_t phase = 0;
-    for (int i = 0; i < nkb; ++i) {
+    for (int i = 0; i < nst; ++i) {
       if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[s], phase))) {
         if (lane == 0) ullm_report(p.status, ULLM_STATUS_TIMEOUT, 132, i);
         abort_flag = 1;
@@ -223,9 +243,11 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint64_t a = desc0 + (uint64_t)(s * (STAGE >> 4)), b = a + (LI_W_BYTES >> 4);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) li_mma(lead, tmem_d, a + 2 * j, b + 2 * j, idesc, i > 0 || j > 0);  // 32 k: 32 bytes along the row
+      for (int j = 0; j < 4 * KB; ++j) {  // 32 k: 32 bytes along the row
+        const uint64_t a = desc0 + (uint64_t)(s * (STAGE >> 4) + j / 4 * (BLOCK >> 4) + j % 4 * 2);
+        li_mma(lead, tmem_d, a, a + (LI_W_BYTES >> 4), idesc, i > 0 || j > 0);
+      }
       umma_commit_warp(lead, lin_smem(&empty_bar[s]));
       if (++s == p.stages) s = 0, phase ^= 1;
     }
@@ -305,7 +327,7 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
   __syncthreads();
   if (abort_flag && threadIdx.x == 0) {
     // a wait ran out: copies may still be on their way into the ring
-    for (int s = 0; s < p.stages && s < nkb; ++s) mbar_wait(&full_bar[s], (((nkb - 1 - s) / p.stages)) & 1);
+    for (int s = 0; s < p.stages && s < nst; ++s) mbar_wait(&full_bar[s], (((nst - 1 - s) / p.stages)) & 1);
   }
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -327,10 +349,11 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
 #define LI_PAIR_STAGES 6
 #define LI_PAIR_TOKENS 256
 
-__device__ __forceinline__ void li_pair_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+__device__ __forceinline__ void li_pair_load(uint32_t lead, uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
+      "{\n .reg .pred q;\n setp.ne.b32 q, %0, 0;\n"
+      " @q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%1], [%2, {%4, %5}], [%3];\n}\n"
+      ::"r"(lead), "r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
       : "memory");
 }
 __device__ __forceinline__ void li_pair_mma(uint32_t lead, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
@@ -421,36 +444,36 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
   pdl_wait();
 
   if (warp == 0) {
-    if (lane == 0) {
-      int s = 0;
-      uint32_t parity = 1;  // a fresh barrier passes a wait on parity 1
-      bool ok = true;
-      for (long long tile = cluster; tile < tiles && ok; tile += clusters) {
-        const int c0 = (int)(tile / t_tiles) * 256 + rank * 128, t0 = (int)(tile % t_tiles) * BN + rank * (BN / 2);
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
-          if (!mbar_wait(&empty_bar[s], parity)) {
-            ullm_report(p.status, ULLM_STATUS_TIMEOUT, 134, kb);
-            abort_flag = 1;
-            ok = false;
-            break;
-          }
-          const uint32_t bar = li_rank_addr(lin_smem(&full_bar[s]), 0), st = lin_smem(ring + s * STAGE);
-          if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * STAGE);
-          li_pair_load(st, &w_map, bar, kb * 128, c0);
-          li_pair_load(st + LI_W_BYTES, &x_map, bar, kb * 128, t0);
-          if (++s == LI_PAIR_STAGES) s = 0, parity ^= 1;
-        }
-      }
-      // (the commits that free the last stages arrive in both blocks: neither ends before)
-      for (int i = 0; i < LI_PAIR_STAGES && ok; ++i) {
-        if (!mbar_wait(&empty_bar[s], parity)) {
-          ullm_report(p.status, ULLM_STATUS_TIMEOUT, 139, i);
+    const uint32_t lead = elect_one(), both = rank == 0 ? lead : 0u;
+    const uint32_t ring0 = lin_smem(ring), full0 = li_rank_addr(lin_smem(&full_bar[0]), 0), own0 = lin_smem(&full_bar[0]);
+    const uint32_t empty0 = lin_smem(&empty_bar[0]);
+    int s = 0;
+    uint32_t parity = 1;  // a fresh barrier passes a wait on parity 1
+    bool ok = true;
+    for (long long tile = cluster; tile < tiles && ok; tile += clusters) {
+      const int c0 = (int)(tile / t_tiles) * 256 + rank * 128, t0 = (int)(tile % t_tiles) * BN + rank * (BN / 2);
+      for (int kb = 0; kb < p.k_blocks; ++kb) {
+        if (!__all_sync(0xffffffffu, mbar_wait_addr(empty0 + s * 8, parity))) {
+          if (lane == 0) ullm_report(p.status, ULLM_STATUS_TIMEOUT, 134, kb);
+          abort_flag = 1;
           ok = false;
+          break;
         }
+        const uint32_t st = ring0 + s * STAGE, bar = full0 + s * 8;
+        li_expect(both, own0 + s * 8, 2 * STAGE);  // (the leader's barrier counts both blocks' bytes)
+        li_pair_load(lead, st, &w_map, bar, kb * 128, c0);
+        li_pair_load(lead, st + LI_W_BYTES, &x_map, bar, kb * 128, t0);
         if (++s == LI_PAIR_STAGES) s = 0, parity ^= 1;
       }
     }
-    __syncwarp();
+    // (the commits that free the last stages arrive in both blocks: neither ends before)
+    for (int i = 0; i < LI_PAIR_STAGES && ok; ++i) {
+      if (!__all_sync(0xffffffffu, mbar_wait_addr(empty0 + s * 8, parity))) {
+        if (lane == 0) ullm_report(p.status, ULLM_STATUS_TIMEOUT, 139, i);
+        ok = false;
+      }
+      if (++s == LI_PAIR_STAGES) s = 0, parity ^= 1;
+    }
   } else if (warp == 1) {
     if (rank == 0) {
       constexpr uint32_t idesc = li_idesc(256, BN);
@@ -544,74 +567,70 @@ static bool li_map(const void* ptr, long long rows, long long cols, long long st
 
 static int g_li_sms = 0;
 
-// Clusters of `ks` blocks that a product of tiles of `nt` tokens is given at most: so many that their blocks come to 4/3 of the SMs, two on
-// some; where a block takes a whole SM, what finds room at once (a GPC's SMs are no multiple of a cluster: 32 clusters of 4 do, 34 take
-// a second round, 96 x 2,057 x 1,104 in 8.6 us for 5.4).
-static int li_clusters_most(int nt, int ks) {
-  if (nt < 64) return 4 * g_li_sms / (3 * ks);
-  return ks == 2 ? g_li_sms * 36 / 74 : ks == 4 ? g_li_sms * 16 / 74 : 0;
+// Whether a product of `tiles` tiles shared by `ks` blocks each has an SM for every block, which then takes a ring of the SM's whole shared
+// memory; the others take half of it, two to an SM.  A GPC's SMs are no multiple of a cluster: 32 clusters of 4 find room at once, 34
+// take a second round (96 x 2,057 x 1,104 in 8.6 us for 5.4).
+static bool li_deep(long long tiles, int ks) {
+  return tiles <= (ks == 1 ? g_li_sms : ks == 2 ? g_li_sms * 36 / 74 : ks == 4 ? g_li_sms * 16 / 74 : 0);
 }
 
 // Which form a product takes: the one that this estimate finds fastest, in ns.  A launch and a tile's end take `start`; a stage of 128 k
-// takes `one` where an SM has one block at a time and `two` where it has two; weights come from memory at 6.4 GB a ms at most (5 through
-// pairs).  Sharing tiles costs two meetings of the cluster and the way of the sums.  The constants are fitted to 247 products (1 to
-// 2,048 tokens, 320 to 24,576 channels, k of 512 to 12,288), each timed in every form: the form chosen here takes 0.7 % more than the
-// fastest one on average, 11 % at most.  What the forms are for, in us beside the nearest alternative:
-//   16, 32, 64 tokens a tile   few tokens: 8 x 24,576 x 4,096 19.8; 64 x 4,096 x 12,288 12.7 (pairs 31)
-//   shared tiles               few tiles: 8 x 4,096 x 4,096 5.8 (alone 9.7), 8 x 2,048 x 8,192 6.0 (alone 16.8)
-//   128 tokens a tile          96 x 24,576 x 4,096 22.7 (64 tokens 31, pairs 27); 384 x 12,288 x 4,096 18.6 (28; 26)
-//   pairs, 256 tokens          512 x 24,576 x 4,096 39 (128 tokens 65); 2,048 x 24,576 x 4,096 128 (248)
+// takes `deep` in a block that has an SM and its ring to itself, else `half`, or `two` for two blocks of an SM; weights come from memory
+// at 5.9 GB a ms (4.9 through pairs), partly beside that.  Sharing tiles costs two meetings of the cluster and the way of the sums.  The
+// constants are fitted to 280 products (1 to 2,048 tokens, 320 to 24,576 channels, k of 512 to 12,288), each timed in every form: the form
+// chosen here takes 0.5 % more than the fastest one on average, 12 % at most.  What the forms are for, in us beside the nearest other:
+//   16, 32, 64 tokens a tile   few tokens: 1 x 6,144 x 4,096 7.0 (shared by two 7.6), 8 x 24,576 x 4,096 19.8; 64 x 6,144 x 4,096 8.5 (9.2)
+//   shared tiles               few tiles: 8 x 4,096 x 12,288 11.0 (alone 14.4), 16 x 512 x 12,288 6.1 (14.0), 64 x 4,096 x 12,288 12.5 (17.7)
+//   128 tokens a tile          96 x 24,576 x 4,096 22.7 (64 tokens 31, pairs 27); 512 x 4,096 x 4,096 10.4 (64 tokens 12.4, pairs 15.4)
+//   pairs, 256 tokens          512 x 24,576 x 4,096 39 (128 tokens 64); 2,048 x 24,576 x 4,096 124 (233)
 struct LiForm {
   int pair, tile, ksplit;
 };
 static LiForm li_choose(int M, int N, int K) {
-  static const int tile[4] = {16, 32, 64, 128}, start[4] = {2700, 2800, 3500, 4000}, one[4] = {250, 240, 260, 270},
-                   two[4] = {400, 300, 365, 465};
+  static const int tile[4] = {16, 32, 64, 128}, start[4] = {1180, 1170, 3430, 3700}, deep[4] = {98, 109, 149, 180},
+                   half[4] = {165, 200, 260, 200}, two[4] = {300, 310, 343, 442};
   const int k_blocks = (K + 127) / 128;
   const long long sms = g_li_sms;
   const double weights = (double)N * K;
   LiForm best = {0, 16, 1};
   double least = 1e300;
   for (int i = 0; i < 4; ++i) {
-    const int nt = tile[i];
+    const int nt = tile[i], kb = nt < 64 ? 2 : 1;  // (blocks of k a stage)
     if ((i > 0 && nt >= 2 * M) || (nt < 64 && nt < M)) continue;
     const long long tiles = (long long)((N + 127) / 128) * ((M + nt - 1) / nt);
     for (int ks = 1; ks <= 8; ks *= 2) {
-      if (ks > 1 && (k_blocks < 2 * ks || tiles > li_clusters_most(nt, ks))) break;
-      const long long blocks = tiles * ks, rounds = blocks / (2 * sms), rest = blocks % (2 * sms);
-      const double stage = (double)rounds * two[i] + (rest == 0 ? 0 : rest <= sms ? one[i] : two[i]);
-      double t = stage * ((k_blocks + ks - 1) / ks);
-      if (t < weights / 6400) t = weights / 6400;
-      t += start[i] + (ks > 1 ? 160 + 24 * (nt < M ? nt : M) : 0);
+      const bool own = li_deep(tiles, ks);
+      if (ks > 1 && (k_blocks < 2 * ks || (!own && (nt >= 64 || ks < 8 || tiles * ks > sms)))) continue;
+      const long long rounds = tiles * ks / (2 * sms), rest = tiles * ks % (2 * sms);
+      const double stage = own ? deep[i] : (double)rounds * two[i] + (rest == 0 ? 0 : rest <= sms ? half[i] : two[i]);
+      const double t = start[i] + hypot(stage * (((k_blocks + kb - 1) / kb + ks - 1) / ks * kb), weights / 5940) +
+                       (ks > 1 ? 1070 + 13 * (nt < M ? nt : M) : 0);
       if (t < least) least = t, best = {0, nt, ks};
     }
   }
   if (M > 64) {
     const long long tiles = (long long)((N + 255) / 256) * ((M + LI_PAIR_TOKENS - 1) / LI_PAIR_TOKENS);
-    double t = (double)((tiles + sms / 2 - 1) / (sms / 2)) * k_blocks * 277;
-    if (t < weights / 5000) t = weights / 5000;
-    if (t + 5680 < least) best = {1, LI_PAIR_TOKENS, 1};
+    const double t = 6050 + hypot((double)((tiles + sms / 2 - 1) / (sms / 2)) * k_blocks * 168, weights / 4950);
+    if (t < least) best = {1, LI_PAIR_TOKENS, 1};
   }
   return best;
 }
 
-template <typename T, int NT>
+template <typename T, int NT, int KB>
 static int li_launch_tc(LiParams p, int ksplit, cudaStream_t st) {
-  constexpr int STAGE = LI_W_BYTES + NT * 128;
-  // Two blocks an SM, or one with a ring of up to 12 stages: where an SM has one block only, and where two rings would be too short.
+  constexpr int STAGE = KB * (LI_W_BYTES + NT * 128);
   constexpr int DEEP = 216 * 1024 / STAGE < LI_MAX_STAGES ? 216 * 1024 / STAGE : LI_MAX_STAGES, HALF = 109 * 1024 / STAGE;
   static_assert((NT < 64 ? HALF : DEEP) * STAGE >= (NT + 32) * 512, "the ring holds a cluster's sums");
   const int n_tiles = (p.N + 127) / 128, m_tiles = (p.M + NT - 1) / NT;
   if (m_tiles > 65535) return ULLM_ERR_UNSUPPORTED;
   static bool set = false;
   if (!set) {
-    if (cudaFuncSetAttribute(linear_int8_tc<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, DEEP * STAGE + 1024) != cudaSuccess)
+    if (cudaFuncSetAttribute(linear_int8_tc<T, NT, KB>, cudaFuncAttributeMaxDynamicSharedMemorySize, DEEP * STAGE + 1024) != cudaSuccess)
       return ULLM_ERR_LAUNCH;
     set = true;
   }
   p.ksplit = ksplit;
-  const long long blocks = (long long)n_tiles * m_tiles * ksplit;
-  p.stages = NT >= 64 && (ksplit > 1 || blocks <= g_li_sms) ? DEEP : HALF;
+  p.stages = li_deep((long long)n_tiles * m_tiles, ksplit) ? DEEP : HALF;
   const int smem = p.stages * STAGE + 1024;
   CUtensorMap w_map, x_map;
   if (!li_map(p.w, p.N, p.K, p.w_stride, 128, &w_map) || !li_map(p.x, p.M, p.K, p.x_stride, NT, &x_map)) return ULLM_ERR_LAUNCH;
@@ -628,7 +647,7 @@ static int li_launch_tc(LiParams p, int ksplit, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g_ullm_pdl ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, linear_int8_tc<T, NT>, w_map, x_map, p) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, linear_int8_tc<T, NT, KB>, w_map, x_map, p) != cudaSuccess) {
     cudaGetLastError();
     return ULLM_ERR_LAUNCH;
   }
@@ -661,10 +680,10 @@ static int li_run(const LiParams& p, cudaStream_t st) {
   }
   const LiForm f = li_choose(p.M, p.N, p.K);
   if (f.pair) return li_launch_pair<T>(p, st);
-  if (f.tile == 16) return li_launch_tc<T, 16>(p, f.ksplit, st);
-  if (f.tile == 32) return li_launch_tc<T, 32>(p, f.ksplit, st);
-  if (f.tile == 64) return li_launch_tc<T, 64>(p, f.ksplit, st);
-  return li_launch_tc<T, 128>(p, f.ksplit, st);
+  if (f.tile == 16) return li_launch_tc<T, 16, 2>(p, f.ksplit, st);
+  if (f.tile == 32) return li_launch_tc<T, 32, 2>(p, f.ksplit, st);
+  if (f.tile == 64) return li_launch_tc<T, 64, 1>(p, f.ksplit, st);
+  return li_launch_tc<T, 128, 1>(p, f.ksplit, st);
 }
 
 static int li_read_sms() {
