@@ -350,3 +350,35 @@ def test_more_than_31_bits_of_elements():
     out = run(x, xs, w, ws, torch.bfloat16)
     for rows in (slice(0, 64), slice(35000, 35064), slice(M - 64, M)):
         check_product(out[rows], *product(x[rows], xs[rows], w, ws))
+
+
+def test_refusals_on_the_gpu():
+    """The same refusals as on the CPU (test_int8_refusals.py), through the checks that run here; nothing is launched or written."""
+    from ullm_b200.csrc.ops import KernelError
+
+    kk = K()
+    x, w = torch.zeros(3, 32, dtype=torch.int8, device=device()), torch.zeros(5, 32, dtype=torch.int8, device=device())
+    xs, ws, out = torch.zeros(3, device=device()), torch.zeros(5, device=device()), torch.full((3, 5), 9.0, device=device())
+    v, gu = torch.zeros(3, 32, device=device()), torch.zeros(3, 64, device=device())
+    before = kk.launches
+    for call in (lambda: kk.linear_int8(v, xs, w, ws, out), lambda: kk.linear_int8(x[:, :16], xs, w, ws, out),
+                 lambda: kk.linear_int8(x, xs[:2], w, ws, out), lambda: kk.linear_int8(x, xs, w, ws.double(), out),
+                 lambda: kk.linear_int8(x, xs, w, ws, out.t()), lambda: kk.linear_int8(x, xs, w, ws, out.double()),
+                 lambda: kk.linear_int8(x, xs, w, ws, out, ws[:4]), lambda: kk.linear_int8(x, xs, w, ws, out, ws.half()),
+                 lambda: kk.linear_int8(x[:1].expand(3, 32), xs, w, ws, out), lambda: kk.linear_int8(x, xs, w.cpu(), ws, out),
+                 lambda: kk.linear_int8(x[0], xs, w, ws, out), lambda: kk.linear_int8(x[:, :0], xs, w[:, :0], ws, out),
+                 lambda: kk.quantize_rows_int8(v.double(), x, xs), lambda: kk.quantize_rows_int8(v, x[:, :31], xs),
+                 lambda: kk.quantize_rows_int8(v, x, xs.cpu()), lambda: kk.quantize_rows_int8(v.t(), x, xs),
+                 lambda: kk.quantize_rows_int8(v[:, :0], x[:, :0], xs),
+                 lambda: kk.act_mul_int8(gu[:, :63], x, xs), lambda: kk.act_mul_int8(gu, x, xs, 2), lambda: kk.act_mul_int8(v, x, xs),
+                 lambda: kk.add_rmsnorm_int8(v, v[:2], torch.ones(32, device=device()), 1e-6, x, xs),
+                 lambda: kk.add_rmsnorm_int8(v, None, torch.ones(31, device=device()), 1e-6, x, xs),
+                 lambda: kk.add_rmsnorm_int8(gu[:, :32], None, torch.ones(32, device=device()), 1e-6, x, xs)):
+        with pytest.raises(KernelError):
+            call()
+    assert (out == 9.0).all() and kk.launches - before <= 8  # (a launcher's own refusal is counted)
+    # no rows: nothing to do
+    assert kk.linear_int8(x[:0], xs[:0], w, ws, out[:0]) is not None and kk.quantize_rows_int8(v[:0], x[:0], xs[:0]) is not None
+    # eps as a whole number, and no weight on a norm's statistics
+    kk.add_rmsnorm_int8(v + 1, None, torch.ones(32, device=device()), 0, x, xs)
+    assert (x == 127).all() and torch.allclose(xs, torch.full_like(xs, 1 / 127))

@@ -51,6 +51,7 @@ class Recorder:
 def face(monkeypatch):
     """The Python faces with their checks as Python writes them, on CPU tensors, in front of a library that records what reaches it."""
     monkeypatch.setattr(ops, "_here", lambda t: True)
+    monkeypatch.setattr(ops, "_at_once", None)
     monkeypatch.setattr(ops, "_rows", PYTHON_ROWS)
     monkeypatch.setattr(ops, "_vector", PYTHON_VECTOR)
     monkeypatch.setattr(ops, "_ptr", lambda t: t)
@@ -124,8 +125,11 @@ def test_tensors_elsewhere():
     """On the CPU, with the checks as they are: the message says where the tensor is."""
     x, q, s = torch.zeros(3, 8), torch.zeros(3, 8, dtype=torch.int8), torch.zeros(3)
     k = object.__new__(ops.Kernels)
-    k.skip_groups, k.timer, k.device_index = frozenset(), None, 0
+    k.skip_groups, k.timer, k.device_index, k.lib, k.status = frozenset(), None, 0, Recorder(), s
     with pytest.raises(ops.KernelError):
         k.quantize_rows_int8(x, q, s)
     native = load_native()
+    launcher = native.bind("ullm_quantize_rows_int8", 1)
+    for args in ((launcher, x, q, s, s), (launcher, x, q, s), (launcher, None, q, s, s), (launcher, x, q, s, None)):
+        assert native.quantize_rows_int8(*args) is None
     assert native.rows(q, torch.int8, 3, 8) == -1 and native.vector(s, torch.float32, 3) is False

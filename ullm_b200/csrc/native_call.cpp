@@ -8,6 +8,9 @@
 //   stream    the current stream's handle
 //   need      a tensor's device, type and layout; what does not hold goes on to the Python check, which says what is wrong
 //   rows      the elements between a matrix's rows, -1 where the tensor is not what a kernel takes there; vector: the same of a vector
+//   quantize_rows_int8, add_rmsnorm_int8, act_mul_int8, linear_int8
+//             the checks and the call of these operators in one, for the smallest of which Python's own (1.6 us) were as long as the kernel;
+//             the launcher's code, or None where a check does not hold (ops.py then says which)
 //   mm        out = x . w^T in bfloat16 by the vendor library, called as `torch.mm` calls it (the same handle, workspace, stream,
 //             algorithm and math mode), without the dispatcher's 4 us; False for what only `torch.mm` should decide
 //
@@ -328,6 +331,137 @@ PyObject* vector(PyObject*, PyObject* const* args, Py_ssize_t n) try {
   return thrown();
 }
 
+// ---- 8-bit rows and products: checks and call in one (their meaning: ops.py) -------------------------------------------------------
+bool held_by(PyObject* o, int device) {
+  if (!THPVariable_Check(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  return t.is_cuda() && t.layout() == at::kStrided && t.get_device() == device;
+}
+// the elements between the rows of a [r, c] matrix of that type (`dense`: a contiguous one), -1 where it is none
+long long stride_of(PyObject* o, at::ScalarType type, int64_t r, int64_t c, bool dense, int device) {
+  if (!held_by(o, device)) return -1;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.scalar_type() != type || t.dim() != 2 || t.size(0) != r || t.size(1) != c || (dense && !t.is_contiguous()) ||
+      (c > 1 && t.stride(1) != 1) || (r > 1 && t.stride(0) < c))
+    return -1;
+  return r > 1 ? t.stride(0) : (c + 15) / 16 * 16;
+}
+bool numbers(PyObject* o, at::ScalarType type, int64_t n, int device) {
+  if (!held_by(o, device)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  return t.scalar_type() == type && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
+}
+int type_code(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1; }
+bool sizes(PyObject* o, int64_t* r, int64_t* c) {
+  if (!THPVariable_Check(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.dim() != 2 || t.layout() != at::kStrided) return false;
+  *r = t.size(0), *c = t.size(1);
+  return *r <= INT_MAX && *c <= INT_MAX;
+}
+// the device that the kernels were set up on, which has to be the current one; -1 else
+int set_up_on(PyObject* status) {
+  if (!THPVariable_Check(status)) return -1;
+  const at::Tensor& t = THPVariable_Unpack(status);
+  return t.is_cuda() && t.get_device() == at::cuda::current_device() ? t.get_device() : -1;
+}
+
+struct Arguments {
+  PyObject* v[16];
+  PyObject* made[16];
+  int n = 0, m = 0;
+  bool fine = true;
+  void add(PyObject* o) { v[n++] = o; }
+  void mine(PyObject* o) {
+    if (o == nullptr) fine = false;
+    else add(made[m++] = o);
+  }
+  void add(long long i) { mine(PyLong_FromLongLong(i)); }
+  void stream() { mine(PyLong_FromVoidPtr(at::cuda::getCurrentCUDAStream().stream())); }
+  PyObject* call(PyObject* launcher) {
+    if (!fine) return nullptr;
+    if (Py_TYPE(launcher) != &LauncherType) {
+      PyErr_SetString(PyExc_TypeError, "the first argument is the operator's launcher");
+      return nullptr;
+    }
+    Launcher* l = reinterpret_cast<Launcher*>(launcher);
+    return l->call(l->fn, v, n);
+  }
+  ~Arguments() {
+    for (int i = 0; i < m; ++i) Py_DECREF(made[i]);
+  }
+};
+
+// (launcher, x, out, scales, status)
+PyObject* quantize_rows_int8(PyObject*, PyObject* const* o, Py_ssize_t n) try {
+  int64_t r, c;
+  if (n != 5 || !sizes(o[1], &r, &c)) Py_RETURN_NONE;
+  const int device = set_up_on(o[4]);
+  const at::ScalarType type = THPVariable_Unpack(o[1]).scalar_type();
+  const long long xs = stride_of(o[1], type, r, c, false, device), os = stride_of(o[2], at::kChar, r, c, false, device);
+  if (device < 0 || type_code(type) < 0 || xs < 0 || os < 0 || !numbers(o[3], at::kFloat, r, device)) Py_RETURN_NONE;
+  Arguments a;
+  a.add(type_code(type)), a.add(o[1]), a.add(xs), a.add(o[2]), a.add(os), a.add(o[3]), a.add(r), a.add(c), a.add(o[4]), a.stream();
+  return a.call(o[0]);
+} catch (...) {
+  return thrown();
+}
+
+// (launcher, x, residual, weight, eps, out, scales, status)
+PyObject* add_rmsnorm_int8(PyObject*, PyObject* const* o, Py_ssize_t n) try {
+  int64_t r, c;
+  if (n != 8 || !sizes(o[1], &r, &c)) Py_RETURN_NONE;
+  const int device = set_up_on(o[7]);
+  const at::ScalarType type = THPVariable_Unpack(o[1]).scalar_type();
+  const long long os = stride_of(o[5], at::kChar, r, c, false, device);
+  if (device < 0 || type_code(type) < 0 || os < 0 || stride_of(o[1], type, r, c, true, device) < 0 ||
+      (o[2] != Py_None && stride_of(o[2], type, r, c, true, device) < 0) || !numbers(o[3], at::kFloat, c, device) ||
+      !numbers(o[6], at::kFloat, r, device) || !PyFloat_Check(o[4]))
+    Py_RETURN_NONE;
+  Arguments a;
+  a.add(type_code(type)), a.add(o[1]), a.add(o[2]), a.add(o[3]), a.add(o[5]), a.add(os), a.add(o[6]), a.add(r), a.add(c), a.add(o[4]),
+      a.add(o[7]), a.stream();
+  return a.call(o[0]);
+} catch (...) {
+  return thrown();
+}
+
+// (launcher, gate_up, out, scales, act, status)
+PyObject* act_mul_int8(PyObject*, PyObject* const* o, Py_ssize_t n) try {
+  int64_t r, c;
+  if (n != 6 || !sizes(o[1], &r, &c) || c % 2 || !PyLong_Check(o[4])) Py_RETURN_NONE;
+  const int device = set_up_on(o[5]);
+  const at::ScalarType type = THPVariable_Unpack(o[1]).scalar_type();
+  const long long os = stride_of(o[2], at::kChar, r, c / 2, false, device);
+  if (device < 0 || type_code(type) < 0 || os < 0 || stride_of(o[1], type, r, c, true, device) < 0 ||
+      !numbers(o[3], at::kFloat, r, device))
+    Py_RETURN_NONE;
+  Arguments a;
+  a.add(type_code(type)), a.add(o[4]), a.add(o[1]), a.add(o[2]), a.add(os), a.add(o[3]), a.add(r), a.add(c / 2), a.add(o[5]), a.stream();
+  return a.call(o[0]);
+} catch (...) {
+  return thrown();
+}
+
+// (launcher, x, x_scales, weight, w_scales, out, bias, status)
+PyObject* linear_int8(PyObject*, PyObject* const* o, Py_ssize_t n) try {
+  int64_t r, k, c, wk;
+  if (n != 8 || !sizes(o[1], &r, &k) || !sizes(o[3], &c, &wk) || !THPVariable_Check(o[5]) || k > 131071) Py_RETURN_NONE;
+  const int device = set_up_on(o[7]);
+  const at::ScalarType type = THPVariable_Unpack(o[5]).scalar_type();
+  const long long xs = stride_of(o[1], at::kChar, r, k, false, device), ws = stride_of(o[3], at::kChar, c, k, false, device);
+  if (device < 0 || type_code(type) < 0 || xs < 0 || ws < 0 || stride_of(o[5], type, r, c, true, device) < 0 ||
+      !numbers(o[2], at::kFloat, r, device) || !numbers(o[4], at::kFloat, c, device) ||
+      (o[6] != Py_None && !numbers(o[6], type, c, device)))
+    Py_RETURN_NONE;
+  Arguments a;
+  a.add(type_code(type)), a.add(o[1]), a.add(xs), a.add(o[2]), a.add(o[3]), a.add(ws), a.add(o[4]), a.add(o[6]), a.add(o[5]), a.add(r),
+      a.add(c), a.add(k), a.add(o[7]), a.stream();
+  return a.call(o[0]);
+} catch (...) {
+  return thrown();
+}
+
 // out [M, N] (bfloat16, or float32 where `wide`) = x [M, K] . w [N, K]^T, on the current stream; the library's status
 int product(void* x, void* w, void* out, int M, int N, int K, int wide) {
   const float one = 1.f, zero = 0.f;
@@ -539,6 +673,10 @@ PyMethodDef methods[] = {
     {"need", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(need)), METH_FASTCALL | METH_KEYWORDS, "checks a tensor"},
     {"rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(rows)), METH_FASTCALL, "the elements between a matrix's rows, or -1"},
     {"vector", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(vector)), METH_FASTCALL, "whether a tensor is such a vector"},
+    {"quantize_rows_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(quantize_rows_int8)), METH_FASTCALL, "checks and calls"},
+    {"add_rmsnorm_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(add_rmsnorm_int8)), METH_FASTCALL, "checks and calls"},
+    {"act_mul_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(act_mul_int8)), METH_FASTCALL, "checks and calls"},
+    {"linear_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(linear_int8)), METH_FASTCALL, "checks and calls"},
     {"stream", stream, METH_NOARGS, "the current stream's handle on the current device"},
     {"set_slow_need", set_slow_need, METH_O, "the check that `need` falls back to"},
     {"mm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(mm)), METH_FASTCALL, "a bfloat16 product by the vendor library"},

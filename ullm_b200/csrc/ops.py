@@ -97,6 +97,7 @@ def _refused(what: str, **tensors) -> None:
 
 # the native forms (native_call.cpp), set when the library is loaded
 _ptr = _need = _stream = _native = None
+_at_once = None  # native_call.cpp where it checks and calls the 8-bit operators in one
 
 
 def _timed(group: str, nbytes=None, skipped=None):
@@ -167,12 +168,13 @@ class _Library:
     """The compiled library: its launchers and queries as calls of native_call.cpp, any other function through ctypes."""
 
     def __init__(self, path: str):
-        global _ptr, _need, _stream, _native, _rows, _vector
+        global _ptr, _need, _stream, _native, _rows, _vector, _at_once
         self._dll = ctypes.CDLL(path)
         _native = calls()
         _native.set_slow_need(_checked)
         _ptr, _need, _stream = _native.ptr, _native.need, _native.stream
         _rows, _vector = _native.rows or _rows, _native.vector or _vector
+        _at_once = _native if _native.quantize_rows_int8 is not None else None
         for name in (*LAUNCHERS, *QUERIES):
             setattr(self, name, _native.bind(name, ctypes.cast(getattr(self._dll, name), c_void_p).value))
 
@@ -808,15 +810,27 @@ class Kernels:
     # the whole numbers nearest to y / s, ties to even.  A row of zeros has the scale 0; a row that holds an infinity or a NaN has the
     # scale NaN (and zeros), so that all that is made of it is NaN.  Rows may lie apart (`int8_rows`): the product takes rows on borders
     # of 16 bytes to the tensor cores and any others to a plain kernel that is ten times slower.
+    #
+    # Each is checked and called by native_call.cpp in one; what does not pass there, and every call while a timer or a measurement
+    # watches, goes through the Python check (`_quantize_rows_int8` and so on), which says what is wrong.
+    def _unwatched(self) -> bool:
+        return _at_once is not None and self.timer is None and not self.skip_groups
+
     @staticmethod
     def int8_rows(rows: int, cols: int, device="cuda") -> torch.Tensor:
         """Room for 8-bit rows on borders of 16 bytes: int8 [rows, cols], contiguous where cols is a multiple of 16."""
         return torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device=device)[:, :cols]
 
-    @_timed("quantize_rows_int8")
     def quantize_rows_int8(self, x, out, scales):
         """out (int8 [T, C]), scales (float32 [T]) <- the rows of x [T, C] in 8 bits.  Rows of x may lie apart (a column range of wider
         ones).  A weight [N, K] is held the same way: one row and one scale per output channel."""
+        if self._unwatched() and _at_once.quantize_rows_int8(self.lib.ullm_quantize_rows_int8, x, out, scales, self.status) == 0:
+            self.launches += 1
+            return out
+        return self._quantize_rows_int8(x, out, scales)
+
+    @_timed("quantize_rows_int8")
+    def _quantize_rows_int8(self, x, out, scales):
         if x.dim() == 2 and x.dtype in _DT and not self._elsewhere(x):
             rows, cols = x.shape
             x_stride, stride = _rows(x, x.dtype, rows, cols), _rows(out, torch.int8, rows, cols)
@@ -827,10 +841,17 @@ class Kernels:
                 return out if code == 0 else self._check(code, f"quantize_rows_int8 (row length {cols})")
         _refused("quantize_rows_int8", x=x, out=out, scales=scales)
 
-    @_timed("add_rmsnorm_int8")
     def add_rmsnorm_int8(self, x, residual, weight, eps: float, out, scales):
         """`add_rmsnorm` with its result in 8 bits: s = x + residual in 32-bit, residual <- s rounded (in place; residual may be None),
         out (int8 [T, C]), scales (float32 [T]) <- the rows s / sqrt(mean(s^2) + eps) * weight."""
+        if self._unwatched() and _at_once.add_rmsnorm_int8(self.lib.ullm_add_rmsnorm_int8, x, residual, weight, eps, out, scales,
+                                                           self.status) == 0:
+            self.launches += 1
+            return out
+        return self._add_rmsnorm_int8(x, residual, weight, eps, out, scales)
+
+    @_timed("add_rmsnorm_int8")
+    def _add_rmsnorm_int8(self, x, residual, weight, eps: float, out, scales):
         dtype = x.dtype
         if x.dim() == 2 and dtype in _DT and x.is_contiguous() and not self._elsewhere(x):
             rows, cols = x.shape
@@ -844,10 +865,16 @@ class Kernels:
                 return out if code == 0 else self._check(code, f"add_rmsnorm_int8 (row length {cols})")
         _refused("add_rmsnorm_int8", x=x, residual=residual, weight=weight, out=out, scales=scales)
 
-    @_timed("act_mul_int8")
     def act_mul_int8(self, gate_up, out, scales, act: int = 0):
         """`act_mul` with its result in 8 bits: out (int8 [T, I]), scales (float32 [T]) <- the rows act(gate) * up of gate_up
         [T, 2 I] = [gate | up], in 32-bit up to there (act 0 silu, 1 gelu_tanh)."""
+        if self._unwatched() and _at_once.act_mul_int8(self.lib.ullm_act_mul_int8, gate_up, out, scales, act, self.status) == 0:
+            self.launches += 1
+            return out
+        return self._act_mul_int8(gate_up, out, scales, act)
+
+    @_timed("act_mul_int8")
+    def _act_mul_int8(self, gate_up, out, scales, act: int = 0):
         dtype = gate_up.dtype
         if gate_up.dim() == 2 and dtype in _DT and gate_up.is_contiguous() and not self._elsewhere(gate_up):
             rows, wide = gate_up.shape
@@ -860,11 +887,18 @@ class Kernels:
                 return out if code == 0 else self._check(code, f"act_mul_int8 (row length {inter}, act {act})")
         _refused("act_mul_int8", gate_up=gate_up, out=out, scales=scales)
 
-    @_timed("linear_int8", lambda x, x_scales, weight, *r: weight.numel())
     def linear_int8(self, x, x_scales, weight, w_scales, out, bias=None):
         """out[t, n] = (sum_k x[t, k] weight[n, k]) * x_scales[t] * w_scales[n] (+ bias[n]): x int8 [T, K], weight int8 [N, K], scales
         float32 [T] and [N], out [T, N] float32, bfloat16 or float16, bias [N] of out's type.  The sums are whole numbers and exact
         (K up to 131,071), the result is formed in 32-bit and rounded once (csrc/linear_int8.cu)."""
+        if self._unwatched() and _at_once.linear_int8(self.lib.ullm_linear_int8, x, x_scales, weight, w_scales, out, bias,
+                                                      self.status) == 0:
+            self.launches += 1
+            return out
+        return self._linear_int8(x, x_scales, weight, w_scales, out, bias)
+
+    @_timed("linear_int8", lambda x, x_scales, weight, *r: weight.numel())
+    def _linear_int8(self, x, x_scales, weight, w_scales, out, bias):
         dtype = out.dtype
         if x.dim() == 2 and weight.dim() == 2 and dtype in _DT and out.is_contiguous() and not self._elsewhere(x):
             (rows, k), cols = x.shape, weight.shape[0]

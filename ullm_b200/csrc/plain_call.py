@@ -25,7 +25,7 @@ class PlainCalls:
     def set_slow_need(self, check) -> None:
         self.need = check
 
-    rows = vector = None  # (the Python checks of ops.py)
+    rows = vector = quantize_rows_int8 = None  # (ops.py checks in Python)
 
     def bind(self, name: str, address: int):
         result, types = (I, LAUNCHERS[name]) if name in LAUNCHERS else QUERIES[name]
