@@ -336,18 +336,19 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
 }
 
 // ---------------------------------------------------------------------------------------------
-// Many tokens.  Two blocks (a cluster of two SMs of one pair, cta_group::2) make tiles of 256 channels by 256 tokens: each holds 128 of
+// Many tokens.  Two blocks (a cluster of two SMs of one pair, cta_group::2) make tiles of 256 channels by BN tokens: each holds 128 of
 // the channels and half of the tokens in shared memory, the leader's instructions read both halves, and each block's tensor memory
-// takes its own 128 channels.  So a block loads 32 KB for the work that takes 48 KB alone, which is what keeps the tensor cores fed
-// from L2.  Persistent: tiles go round the clusters, tokens fastest (the weights then come from memory once), and
-// two accumulators let a tile's end run beside the next one's products.
+// takes its own 128 channels.  With 256 tokens a block loads 32 KB for the work that takes 48 KB alone, which is what keeps the tensor
+// cores fed from L2.  Persistent: tiles go round the clusters, tokens fastest (the weights then come from memory once), and two
+// accumulators let a tile's end run beside the next one's products.  Tiles of 128 and 192 tokens are for products whose tiles of 256 would
+// leave SMs idle in the last round, or take one round more: a round of 74 tiles costs 11.0 us at k = 4,096 with 256 tokens, 7.2 with 192.
 //
 // Barriers: a stage is full when the bytes of both blocks have come (the leader's barrier counts them all); an instruction group's
 // commit frees the stage in both blocks, and tells both that an accumulator is complete; the eight finishing warps of both tell the
 // leader that it is drained.
 // ---------------------------------------------------------------------------------------------
-#define LI_PAIR_STAGES 6
-#define LI_PAIR_TOKENS 256
+constexpr int li_pair_stage(int tokens) { return LI_W_BYTES + tokens / 2 * 128; }
+constexpr int li_pair_stages(int tokens) { return 200 * 1024 / li_pair_stage(tokens); }  // (8, 7, 6)
 
 __device__ __forceinline__ void li_pair_load(uint32_t lead, uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
   asm volatile(
@@ -399,12 +400,12 @@ __device__ __forceinline__ void li_tmem_ld32(uint32_t taddr, int (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-template <typename T>
+template <typename T, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LI_THREADS)
 linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const LiParams p) {
-  constexpr int BN = LI_PAIR_TOKENS, STAGE = LI_W_BYTES + BN / 2 * 128;
+  constexpr int STAGE = li_pair_stage(BN), STAGES = li_pair_stages(BN), COLUMNS = BN > 128 ? 512 : 256;
   extern __shared__ unsigned char li_smem_raw[];
-  __shared__ __align__(8) uint64_t full_bar[LI_PAIR_STAGES], empty_bar[LI_PAIR_STAGES], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag, go[2];
   __shared__ __align__(16) float xs_s[2][BN];  // the token scales of a tile
@@ -416,7 +417,7 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int s = 0; s < LI_PAIR_STAGES; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
@@ -432,7 +433,7 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
   // Allocating for a pair takes both blocks: what one asks of the other's SM is lost for good where that block has not started yet, or
   // has ended.  So it stands behind the cluster's first meeting, and giving back in front of its last one.
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lin_smem(&tmem_slot)), "r"(2 * BN)
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(lin_smem(&tmem_slot)), "r"(COLUMNS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     pdl_launch_dependents();  // (only now: a kernel behind this one must not hold tensor memory that this one waits for)
@@ -463,16 +464,16 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
         li_expect(both, own0 + s * 8, 2 * STAGE);  // (the leader's barrier counts both blocks' bytes)
         li_pair_load(lead, st, &w_map, bar, kb * 128, c0);
         li_pair_load(lead, st + LI_W_BYTES, &x_map, bar, kb * 128, t0);
-        if (++s == LI_PAIR_STAGES) s = 0, parity ^= 1;
+        if (++s == STAGES) s = 0, parity ^= 1;
       }
     }
     // (the commits that free the last stages arrive in both blocks: neither ends before)
-    for (int i = 0; i < LI_PAIR_STAGES && ok; ++i) {
+    for (int i = 0; i < STAGES && ok; ++i) {
       if (!__all_sync(0xffffffffu, mbar_wait_addr(empty0 + s * 8, parity))) {
         if (lane == 0) ullm_report(p.status, ULLM_STATUS_TIMEOUT, 139, i);
         ok = false;
       }
-      if (++s == LI_PAIR_STAGES) s = 0, parity ^= 1;
+      if (++s == STAGES) s = 0, parity ^= 1;
     }
   } else if (warp == 1) {
     if (rank == 0) {
@@ -503,7 +504,7 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
 #pragma unroll
           for (int j = 0; j < 4; ++j) li_pair_mma(lead, d, a + 2 * j, b + 2 * j, idesc, kb > 0 || j > 0);
           li_pair_commit(lead, lin_smem(&empty_bar[s]));
-          if (++s == LI_PAIR_STAGES) s = 0, phase ^= 1;
+          if (++s == STAGES) s = 0, phase ^= 1;
         }
         if (ok) li_pair_commit(lead, lin_smem(&acc_full[buf]));
       }
@@ -543,14 +544,14 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
   if (abort_flag && rank == 0 && threadIdx.x == 0) {
     // a wait ran out: copies may still be on their way into either block's ring, whose bytes the leader's barriers count
     const long long mine = tiles > cluster ? ((tiles - 1 - cluster) / clusters + 1) * p.k_blocks : 0;
-    for (int s = 0; s < LI_PAIR_STAGES && s < mine; ++s) mbar_wait(&full_bar[s], (uint32_t)((mine - 1 - s) / LI_PAIR_STAGES) & 1);
+    for (int s = 0; s < STAGES && s < mine; ++s) mbar_wait(&full_bar[s], (uint32_t)((mine - 1 - s) / STAGES) & 1);
   }
   __syncthreads();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   li_cluster_sync();  // nobody arrives at this block's barriers any more, or reads its ring
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_d), "r"(2 * BN) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_d), "r"(COLUMNS) : "memory");
   }
   li_cluster_sync();  // (see the allocation)
 }
@@ -576,19 +577,23 @@ static bool li_deep(long long tiles, int ks) {
 
 // Which form a product takes: the one that this estimate finds fastest, in ns.  A launch and a tile's end take `start`; a stage of 128 k
 // takes `deep` in a block that has an SM and its ring to itself, else `half`, or `two` for two blocks of an SM; weights come from memory
-// at 5.9 GB a ms (4.9 through pairs), partly beside that.  Sharing tiles costs two meetings of the cluster and the way of the sums.  The
-// constants are fitted to 280 products (1 to 2,048 tokens, 320 to 24,576 channels, k of 512 to 12,288), each timed in every form: the form
-// chosen here takes 0.5 % more than the fastest one on average, 12 % at most.  What the forms are for, in us beside the nearest other:
-//   16, 32, 64 tokens a tile   few tokens: 1 x 6,144 x 4,096 7.0 (shared by two 7.6), 8 x 24,576 x 4,096 19.8; 64 x 6,144 x 4,096 8.5 (9.2)
-//   shared tiles               few tiles: 8 x 4,096 x 12,288 11.0 (alone 14.4), 16 x 512 x 12,288 6.1 (14.0), 64 x 4,096 x 12,288 12.5 (17.7)
-//   128 tokens a tile          96 x 24,576 x 4,096 22.7 (64 tokens 31, pairs 27); 512 x 4,096 x 4,096 10.4 (64 tokens 12.4, pairs 15.4)
-//   pairs, 256 tokens          512 x 24,576 x 4,096 39 (128 tokens 64); 2,048 x 24,576 x 4,096 124 (233)
+// at 6.6 GB a ms, partly beside that.  Sharing tiles costs two meetings of the cluster and the way of the sums.  The constants are fitted
+// to 280 products (1 to 2,048 tokens, 320 to 24,576 channels, k of 512 to 12,288), each timed in every form: the form chosen here takes
+// 0.5 % more than the fastest one on average, 12 % at most, and the estimate is 12 % off on average.  What the forms are for, in us
+// beside the nearest other:
+//   16, 32, 64 tokens a tile   few tokens: 1 x 6,144 x 4,096 7.0 (shared by two 7.6), 64 x 6,144 x 4,096 8.6 (9.2)
+//   shared tiles               few tiles: 8 x 4,096 x 12,288 10.8 (alone 14.3), 16 x 512 x 12,288 5.4 (12.3), 64 x 4,096 x 12,288 12.5 (18.1)
+//   128 tokens a tile          96 x 24,576 x 4,096 22.5 (64 tokens 30.6, pairs 24); 512 x 4,096 x 4,096 10.4 (pairs 11.0)
+//   pairs, 128 tokens          256 x 24,576 x 4,096 27.1 (128 alone 37, 256 in pairs 29.8)
+//   pairs, 192 tokens          512 x 6,144 x 4,096 13.5 (128 in pairs 16.4); 768 x 4,096 x 12,288 28.0 (256 in pairs 34.8)
+//   pairs, 256 tokens          512 x 24,576 x 4,096 38.5 (192 tokens 41, 128 alone 64); 2,048 x 24,576 x 4,096 126 (133, 235)
 struct LiForm {
   int pair, tile, ksplit;
 };
 static LiForm li_choose(int M, int N, int K) {
-  static const int tile[4] = {16, 32, 64, 128}, start[4] = {1180, 1170, 3430, 3700}, deep[4] = {98, 109, 149, 180},
-                   half[4] = {165, 200, 260, 200}, two[4] = {300, 310, 343, 442};
+  static const int tile[4] = {16, 32, 64, 128}, start[4] = {1930, 2250, 2900, 3200}, deep[4] = {101, 112, 157, 204},
+                   half[4] = {152, 200, 348, 276}, two[4] = {291, 287, 348, 456};
+  static const int pair_tile[3] = {128, 192, 256}, pair_start[3] = {5210, 4030, 4470}, pair_block[3] = {182, 257, 293};
   const int k_blocks = (K + 127) / 128;
   const long long sms = g_li_sms;
   const double weights = (double)N * K;
@@ -603,15 +608,15 @@ static LiForm li_choose(int M, int N, int K) {
       if (ks > 1 && (k_blocks < 2 * ks || (!own && (nt >= 64 || ks < 8 || tiles * ks > sms)))) continue;
       const long long rounds = tiles * ks / (2 * sms), rest = tiles * ks % (2 * sms);
       const double stage = own ? deep[i] : (double)rounds * two[i] + (rest == 0 ? 0 : rest <= sms ? half[i] : two[i]);
-      const double t = start[i] + hypot(stage * (((k_blocks + kb - 1) / kb + ks - 1) / ks * kb), weights / 5940) +
-                       (ks > 1 ? 1070 + 13 * (nt < M ? nt : M) : 0);
+      const double t = start[i] + hypot(stage * (((k_blocks + kb - 1) / kb + ks - 1) / ks * kb), weights / 6600) +
+                       (ks > 1 ? 1200 + 14 * (nt < M ? nt : M) : 0);
       if (t < least) least = t, best = {0, nt, ks};
     }
   }
-  if (M > 64) {
-    const long long tiles = (long long)((N + 255) / 256) * ((M + LI_PAIR_TOKENS - 1) / LI_PAIR_TOKENS);
-    const double t = 6050 + hypot((double)((tiles + sms / 2 - 1) / (sms / 2)) * k_blocks * 168, weights / 4950);
-    if (t < least) best = {1, LI_PAIR_TOKENS, 1};
+  for (int i = 0; i < 3 && M > 64; ++i) {
+    const long long tiles = (long long)((N + 255) / 256) * ((M + pair_tile[i] - 1) / pair_tile[i]);
+    const double t = pair_start[i] + hypot((double)((tiles + sms / 2 - 1) / (sms / 2)) * k_blocks * pair_block[i], weights / 6600);
+    if (t < least) least = t, best = {1, pair_tile[i], 1};
   }
   return best;
 }
@@ -654,13 +659,12 @@ static int li_launch_tc(LiParams p, int ksplit, cudaStream_t st) {
   return ULLM_OK;
 }
 
-template <typename T>
+template <typename T, int BN>
 static int li_launch_pair(const LiParams& p, cudaStream_t st) {
-  constexpr int BN = LI_PAIR_TOKENS;
-  const int smem = LI_PAIR_STAGES * (LI_W_BYTES + BN / 2 * 128) + 1024;
+  const int smem = li_pair_stages(BN) * li_pair_stage(BN) + 1024;
   static bool set = false;
   if (!set) {
-    if (cudaFuncSetAttribute(linear_int8_pair<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    if (cudaFuncSetAttribute(linear_int8_pair<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return ULLM_ERR_LAUNCH;
     set = true;
   }
@@ -668,7 +672,7 @@ static int li_launch_pair(const LiParams& p, cudaStream_t st) {
   const int clusters = (int)(tiles < g_li_sms / 2 ? tiles : g_li_sms / 2);
   CUtensorMap w_map, x_map;
   if (!li_map(p.w, p.N, p.K, p.w_stride, 128, &w_map) || !li_map(p.x, p.M, p.K, p.x_stride, BN / 2, &x_map)) return ULLM_ERR_LAUNCH;
-  return ullm_launch_kernel(linear_int8_pair<T>, dim3(2 * clusters), dim3(LI_THREADS), smem, st, w_map, x_map, p);
+  return ullm_launch_kernel(linear_int8_pair<T, BN>, dim3(2 * clusters), dim3(LI_THREADS), smem, st, w_map, x_map, p);
 }
 
 template <typename T>
@@ -679,7 +683,9 @@ static int li_run(const LiParams& p, cudaStream_t st) {
     return ullm_launch_kernel(linear_int8_plain<T>, dim3((p.N + 31) / 32, (p.M + 31) / 32), dim3(256), 0, st, p);
   }
   const LiForm f = li_choose(p.M, p.N, p.K);
-  if (f.pair) return li_launch_pair<T>(p, st);
+  if (f.pair && f.tile == 128) return li_launch_pair<T, 128>(p, st);
+  if (f.pair && f.tile == 192) return li_launch_pair<T, 192>(p, st);
+  if (f.pair) return li_launch_pair<T, 256>(p, st);
   if (f.tile == 16) return li_launch_tc<T, 16, 2>(p, f.ksplit, st);
   if (f.tile == 32) return li_launch_tc<T, 32, 2>(p, f.ksplit, st);
   if (f.tile == 64) return li_launch_tc<T, 64, 1>(p, f.ksplit, st);
