@@ -195,6 +195,17 @@ def test_rows_anywhere(M, N, k, pad):
     check_product(run(x[:, 1:], xs, w[:, 1:], ws, torch.bfloat16), *product(x[:, 1:], xs, w[:, 1:], ws)) if k > 1 else None
 
 
+# more tokens than a grid has rows of tiles: pairs that go round (rows on borders of 16 bytes), the plain kernel's blocks that go round
+@pytest.mark.parametrize("M,N,k", [(65535 * 128 + 300, 3, 16), (65535 * 32 + 100, 5, 3)])
+def test_many_tokens(M, N, k):
+    x, w = (torch.randint(-128, 128, (n, k), dtype=torch.int8, generator=gen(n % 997), device=device()) for n in (M, N))
+    xs, ws = torch.ones(M, device=device()), torch.ones(N, device=device())
+    out = torch.full((M, N), 0.5, device=device())
+    K().linear_int8(x, xs, w, ws, out)
+    sums = sum(x[:, i:i + 1].int() * w[:, i].int() for i in range(k))  # (whole numbers below 2^24)
+    assert torch.equal(out, sums.float())
+
+
 @pytest.mark.parametrize("pad", [0, 1])
 def test_largest_sums(pad):
     """k of 131,071 with -128 everywhere: 2^14 k is below 2^31 by 16,384."""

@@ -64,39 +64,39 @@ __global__ void __launch_bounds__(256) linear_int8_plain(const LiParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const int n0 = blockIdx.x * 32;
-  const long long m0 = (long long)blockIdx.y * 32;
   const int tn = threadIdx.x & 31, tm = threadIdx.x >> 5;  // a thread: column tn, rows tm, tm + 8, ...
-  int acc[4] = {0, 0, 0, 0};
-  for (int k0 = 0; k0 < p.K; k0 += 64) {
-    for (int i = threadIdx.x; i < 32 * 16 * 2; i += 256) {
-      const bool of_w = i >= 512;
-      const int r = (i >> 4) & 31, q = i & 15, k = k0 + q * 4;
-      const long long row = of_w ? n0 + r : m0 + r;
-      const signed char* src = (of_w ? p.w + row * p.w_stride : p.x + row * p.x_stride) + k;
-      uint32_t v = 0;
-      if (row < (of_w ? p.N : p.M)) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (k + e < p.K) v |= (uint32_t)(unsigned char)src[e] << (8 * e);
-      }
-      (of_w ? ws : xs)[r][q] = (int)v;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < 16; ++q) {
-      const int b = ws[tn][q];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = __dp4a(xs[tm + 8 * i][q], b, acc[i]);
-    }
-    __syncthreads();
-  }
   const int n = n0 + tn;
-  if (n >= p.N) return;
-  const float ws_n = p.w_scales[n], bias = p.bias != nullptr ? to_f32(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
+  const float ws_n = n < p.N ? p.w_scales[n] : 0.f, bias = n < p.N && p.bias != nullptr ? to_f32(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
+  for (long long m0 = (long long)blockIdx.y * 32; m0 < p.M; m0 += (long long)gridDim.y * 32) {
+    int acc[4] = {0, 0, 0, 0};
+    for (int k0 = 0; k0 < p.K; k0 += 64) {
+      for (int i = threadIdx.x; i < 32 * 16 * 2; i += 256) {
+        const bool of_w = i >= 512;
+        const int r = (i >> 4) & 31, q = i & 15, k = k0 + q * 4;
+        const long long row = of_w ? n0 + r : m0 + r;
+        const signed char* src = (of_w ? p.w + row * p.w_stride : p.x + row * p.x_stride) + k;
+        uint32_t v = 0;
+        if (row < (of_w ? p.N : p.M)) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long m = m0 + tm + 8 * i;
-    if (m < p.M) reinterpret_cast<T*>(p.out)[m * p.N + n] = li_result<T>(acc[i], p.x_scales[m], ws_n, bias);
+          for (int e = 0; e < 4; ++e)
+            if (k + e < p.K) v |= (uint32_t)(unsigned char)src[e] << (8 * e);
+        }
+        (of_w ? ws : xs)[r][q] = (int)v;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const int b = ws[tn][q];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = __dp4a(xs[tm + 8 * i][q], b, acc[i]);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long m = m0 + tm + 8 * i;
+      if (m < p.M && n < p.N) reinterpret_cast<T*>(p.out)[m * p.N + n] = li_result<T>(acc[i], p.x_scales[m], ws_n, bias);
+    }
   }
 }
 
@@ -601,7 +601,7 @@ static LiForm li_choose(int M, int N, int K) {
   double least = 1e300;
   for (int i = 0; i < 4; ++i) {
     const int nt = tile[i], kb = nt < 64 ? 2 : 1;  // (blocks of k a stage)
-    if ((i > 0 && nt >= 2 * M) || (nt < 64 && nt < M)) continue;
+    if ((i > 0 && nt >= 2ll * M) || (nt < 64 && nt < M) || (M - 1) / nt >= 65535) continue;  // (a grid has 65,535 rows; pairs go round)
     const long long tiles = (long long)((N + 127) / 128) * ((M + nt - 1) / nt);
     for (int ks = 1; ks <= 8; ks *= 2) {
       const bool own = li_deep(tiles, ks);
@@ -627,7 +627,6 @@ static int li_launch_tc(LiParams p, int ksplit, cudaStream_t st) {
   constexpr int DEEP = 216 * 1024 / STAGE < LI_MAX_STAGES ? 216 * 1024 / STAGE : LI_MAX_STAGES, HALF = 109 * 1024 / STAGE;
   static_assert((NT < 64 ? HALF : DEEP) * STAGE >= (NT + 32) * 512, "the ring holds a cluster's sums");
   const int n_tiles = (p.N + 127) / 128, m_tiles = (p.M + NT - 1) / NT;
-  if (m_tiles > 65535) return ULLM_ERR_UNSUPPORTED;
   static bool set = false;
   if (!set) {
     if (cudaFuncSetAttribute(linear_int8_tc<T, NT, KB>, cudaFuncAttributeMaxDynamicSharedMemorySize, DEEP * STAGE + 1024) != cudaSuccess)
@@ -679,8 +678,7 @@ template <typename T>
 static int li_run(const LiParams& p, cudaStream_t st) {
   const bool aligned = (((uintptr_t)p.x | (uintptr_t)p.w | (uintptr_t)p.x_stride | (uintptr_t)p.w_stride) & 15) == 0;
   if (!aligned) {
-    if ((p.M + 31ll) / 32 > 65535) return ULLM_ERR_UNSUPPORTED;
-    return ullm_launch_kernel(linear_int8_plain<T>, dim3((p.N + 31) / 32, (p.M + 31) / 32), dim3(256), 0, st, p);
+    return ullm_launch_kernel(linear_int8_plain<T>, dim3((p.N + 31) / 32, p.M <= 65535 * 32 ? (p.M + 31) / 32 : 65535), dim3(256), 0, st, p);
   }
   const LiForm f = li_choose(p.M, p.N, p.K);
   if (f.pair && f.tile == 128) return li_launch_pair<T, 128>(p, st);
@@ -710,7 +708,7 @@ extern "C" int ullm_linear_int8_form(int M, int N, int K) {
 // dtype: of out and bias.  Strides in bytes, at least K.
 extern "C" int ullm_linear_int8(int dtype, const void* x, long long x_stride, const void* x_scales, const void* w, long long w_stride,
                                 const void* w_scales, const void* bias, void* out, int M, int N, int K, int* status, void* stream) {
-  if (M < 0 || N <= 0 || N > (1 << 30) || K <= 0 || K > LI_MAX_K || x_stride < K || w_stride < K) return ULLM_ERR_BAD_SIZE;
+  if (M < 0 || M > (1 << 30) || N <= 0 || N > (1 << 30) || K <= 0 || K > LI_MAX_K || x_stride < K || w_stride < K) return ULLM_ERR_BAD_SIZE;
   if (dtype != ULLM_DTYPE_F32 && dtype != ULLM_DTYPE_BF16 && dtype != ULLM_DTYPE_F16) return ULLM_ERR_BAD_DTYPE;
   if (M == 0) return ULLM_OK;
   if (li_read_sms() <= 0) return ULLM_ERR_LAUNCH;
