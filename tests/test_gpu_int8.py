@@ -89,6 +89,57 @@ def test_norm(rows, cols, pad, with_residual, dtype):
     untouched()
 
 
+def placed(x, offset):
+    """x [rows, cols] contiguous in memory that begins `offset` elements behind a border of 16 bytes, and a check of what lies around."""
+    n, wide = x.numel(), torch.full((x.numel() + 64,), 7.0, dtype=x.dtype, device=device())
+    held = wide[16 + offset:16 + offset + n].view(x.shape)
+    held.copy_(x)
+
+    def untouched():
+        assert (wide[:16 + offset] == 7.0).all() and (wide[16 + offset + n:] == 7.0).all()
+
+    return held, untouched
+
+
+# rows of any length in memory at any place, their 8 bits on borders of 16 bytes: a group and less; warps' edges; several groups of a thread
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (9, 3), (9, 7), (17, 9), (9, 15), (17, 33), (9, 255), (17, 257), (9, 259), (33, 1003), (17, 2041), (9, 4095),
+                                       (9, 8191), (5, 9001), (3, 16387), (3, 32767), (2, 32769), (900, 263), (800, 2043), (700, 4101), (140, 1003), (2000, 531), (70, 2041), (9, 5000),
+                                       (5, 4096), (3, 8200)])
+def test_rows_of_any_length(rows, cols, dtype):
+    g = gen(rows * 7 + cols)
+    x, res = rows_of(g, rows, cols, dtype), rows_of(g, rows, cols, dtype)
+    gu, weight = rows_of(g, rows, 2 * cols, dtype), 1 + 0.3 * torch.randn(cols, generator=g, device=device())
+    y, total, (z, size) = normed(x, res, weight, 1e-6), (x.float() + res.float()).to(dtype), gated(gu, 0)
+    wide = -(-cols // 16) * 16 - cols
+    rel = 2.0 ** -22 * (size.abs() + 3)
+    for offset, other in ((0, 0), (1, 3), (5, 5), (6, 2), (3, 0), (0, 7)):
+        q, untouched = room(rows, cols, wide)
+        scales = torch.full((rows,), 9.0, device=device())
+        a, around = placed(x, offset)
+        K().quantize_rows_int8(a, q, scales)
+        check_rows(q, scales, x.double(), 0.0, 2.0 ** -24 * 1.01)
+        b, around_b = placed(res, other)
+        K().add_rmsnorm_int8(a, b, weight, 1e-6, q, scales)
+        check_rows(q, scales, y, 2.0 ** -23, 2.0 ** -24 * ((cols / 1024 + 40) / 2 + 10))
+        assert torch.equal(b, total) and torch.equal(a, x)
+        c, around_c = placed(gu, offset)
+        K().act_mul_int8(c, q, scales)
+        check_rows(q, scales, z, rel, float(rel.max()))
+        for check in (untouched, around, around_b, around_c):
+            check()
+
+
+def test_a_residual_that_is_the_input():
+    for cols in (4096, 2043):
+        x = rows_of(gen(cols), 9, cols, torch.bfloat16)
+        once, weight, scales = x.clone(), torch.ones(cols, device=device()), torch.empty(9, device=device())
+        q = K().int8_rows(9, cols)
+        K().add_rmsnorm_int8(x, x, weight, 1e-6, q, scales)
+        check_rows(q, scales, normed(once, once, weight, 1e-6), 2.0 ** -23, 2.0 ** -24 * 40)
+        assert torch.equal(x, (once.float() * 2).to(torch.bfloat16))
+
+
 def test_ties_go_to_even():
     """A row whose largest element is 127 has the scale 1: what lies between two whole numbers goes to the even one."""
     x = torch.zeros(2, 256, device=device())

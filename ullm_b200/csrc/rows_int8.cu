@@ -19,7 +19,8 @@
 // The work is bound by memory.  Two forms:
 //   rows_int8_kernel   a block takes one row and holds it in registers between the reduction and the store (PER groups of VEC
 //                      neighbouring elements per thread, all loads in flight together); rows too long for that are read a second
-//                      time.  Few rows, and rows that do not come in pieces of 16 bytes.
+//                      time.  Few rows, and rows that do not come in pieces of 16 bytes: pieces shifted into place, or element by
+//                      element.
 //   rows_int8_stream   blocks that stay and take one row after the other, the next rows on their way into shared memory (bulk copies)
 //                      while one is worked on.  Many rows.
 #include "tcgen05_util.cuh"
@@ -38,7 +39,7 @@ struct RqParams {
   int cols;
   int act;                // RQ_ACT: 0 silu, 1 gelu_tanh
   float eps;
-  int rows;               // (rows_int8_stream)
+  int rows;
   int* status;
 };
 
@@ -95,6 +96,74 @@ __device__ __forceinline__ float rq_scale(const RqRow& r, float rstd) {
   return r.keep ? rstd * r.most / 127.f : __uint_as_float(0x7fc00000u);
 }
 
+// ---- rows that do not come in pieces of 16 bytes (ANY): a thread's group lies on its place of the row, wherever that is in memory ----
+// Two neighbouring pieces hold it; a selection of words and a shift bring it into place.
+template <typename T>
+__device__ __forceinline__ int rq_off(const T* at) {  // elements since the last border of 16 bytes
+  return (int)(((uintptr_t)at & 15) / sizeof(T));
+}
+template <int WORDS>  // w[i] <- the word that lies `bytes` (0 to 15) behind w[i]'s first, i < 4
+__device__ __forceinline__ void rq_shift(uint32_t (&w)[WORDS], int bytes) {
+  if (bytes & 8) {
+#pragma unroll
+    for (int i = 0; i + 2 < WORDS; ++i) w[i] = w[i + 2];
+  }
+  if (bytes & 4) {
+#pragma unroll
+    for (int i = 0; i + 1 < WORDS; ++i) w[i] = w[i + 1];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (bytes & 3) * 8);
+}
+// v <- at[0 .. VEC) of a row that has `left` elements from there on, zeros behind them.  The rows' memory has `before` elements in front of
+// `at` and `behind` from there on: pieces that it does not hold whole (at the first row's begin and the last row's end) are not read, but
+// their elements one by one.
+template <typename T, int VEC>
+__device__ __forceinline__ void rq_read(const T* at, long long before, long long behind, int left, float (&v)[VEC]) {
+  const int off = rq_off(at);
+  if (before >= off && behind >= 2 * VEC - off) {
+    const uint4 a = *reinterpret_cast<const uint4*>(at - off), b = *reinterpret_cast<const uint4*>(at - off + VEC);
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    rq_shift(w, off * (int)sizeof(T));
+    const uint4 u = make_uint4(w[0], w[1], w[2], w[3]);
+    const T* h = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = i < left ? to_f32(h[i]) : 0.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = i < left ? to_f32(at[i]) : 0.f;
+  }
+}
+// at[0 .. left) <- v rounded, by a whole warp whose lanes hold neighbouring groups: the piece that a group begins in is stored with the last
+// elements of the group in front, where the same warp holds both and the row all of the piece
+template <typename T, int VEC>
+__device__ __forceinline__ void rq_store_any(T* at, int left, const float (&v)[VEC]) {
+  const int off = rq_off(at), lane = threadIdx.x & 31;
+  uint4 u;
+  T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) e[i] = from_f32<T>(v[i]);
+  uint32_t w[8];
+  w[4] = u.x, w[5] = u.y, w[6] = u.z, w[7] = u.w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __shfl_up_sync(0xffffffffu, w[4 + i], 1);
+  // a piece begins `off` elements in front of its group: VEC - off elements into the group before
+  const bool mine = lane > 0 && left >= VEC - off, next = lane < 31 && left >= 2 * VEC - off;
+  if (off == 0) {
+    if (left >= VEC) {
+      *reinterpret_cast<uint4*>(at) = u;
+      return;
+    }
+  } else if (mine) {
+    rq_shift(w, 16 - off * (int)sizeof(T));
+    *reinterpret_cast<uint4*>(at - off) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (next) return;
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+    if (i < left && (off == 0 || (i < VEC - off ? !mine : !next))) at[i] = e[i];
+}
+
 // VEC values of one place of a row; RQ_NORM: unrounded sums in s beside v = s * w
 template <typename T, int KIND, int VEC>
 __device__ __forceinline__ void rq_load(const RqParams& p, const T* x, const T* res, int c, float (&v)[VEC], float (&s)[VEC]) {
@@ -118,6 +187,36 @@ __device__ __forceinline__ void rq_load(const RqParams& p, const T* x, const T* 
     for (int i = 0; i < VEC; ++i) v[i] *= s[i];
   }
 }
+// the same of rows anywhere
+template <typename T, int KIND, int VEC>
+__device__ __forceinline__ void rq_load_any(const RqParams& p, long long row, const T* x, const T* res, int c, float (&v)[VEC], float (&s)[VEC]) {
+  const int left = p.cols - c;
+  const long long begin = row * p.x_stride + c, end = (p.rows - 1) * p.x_stride + (KIND == RQ_ACT ? 2ll : 1ll) * p.cols;
+  rq_read<T, VEC>(x + c, begin, end - begin, left, v);
+  if constexpr (KIND == RQ_ACT) {
+    rq_read<T, VEC>(x + p.cols + c, begin + p.cols, end - begin - p.cols, left, s);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = rq_gate(v[i], p.act) * s[i];
+  }
+  if constexpr (KIND == RQ_NORM) {
+    if (res != nullptr) {
+      rq_read<T, VEC>(res + c, row * p.cols + c, (p.rows - row) * p.cols - c, left, s);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s[i] += v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s[i] = v[i];
+    }
+    if (left >= VEC) {
+      load_vec32<VEC>(p.weight + c, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = i < left ? p.weight[c + i] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] *= s[i];
+  }
+}
 template <int KIND, int VEC>
 __device__ __forceinline__ void rq_account(const float (&v)[VEC], const float (&s)[VEC], float& sum, float& top) {
 #pragma unroll
@@ -127,7 +226,7 @@ __device__ __forceinline__ void rq_account(const float (&v)[VEC], const float (&
   }
 }
 template <int VEC>
-__device__ __forceinline__ void rq_store(const RqRow& r, signed char* out, const float (&v)[VEC]) {
+__device__ __forceinline__ void rq_store(const RqRow& r, signed char* out, const float (&v)[VEC], int left = VEC) {
   uint32_t q[VEC];
   if (r.tiny) {
 #pragma unroll
@@ -137,22 +236,26 @@ __device__ __forceinline__ void rq_store(const RqRow& r, signed char* out, const
     for (int i = 0; i < VEC; ++i) q[i] = __float_as_uint(fmaf(v[i], r.mul, 12582912.f));
   }
   if constexpr (VEC % 4 == 0) {
-    uint32_t w[VEC / 4];
+    if (left >= VEC) {
+      uint32_t w[VEC / 4];
 #pragma unroll
-    for (int i = 0; i < VEC / 4; ++i)
-      w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410) & r.keep;
-    if constexpr (VEC == 8)
-      *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
-    else
-      *reinterpret_cast<uint32_t*>(out) = w[0];
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) out[i] = (signed char)(q[i] & r.keep & 0xff);
+      for (int i = 0; i < VEC / 4; ++i)
+        w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410) & r.keep;
+      if constexpr (VEC == 8)
+        *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+      else
+        *reinterpret_cast<uint32_t*>(out) = w[0];
+      return;
+    }
   }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+    if (i < left) out[i] = (signed char)(q[i] & r.keep & 0xff);
 }
 
-// PER > 0: the row in registers, PER * VEC * blockDim >= cols.  PER = 0: any length, read twice.
-template <typename T, int KIND, int VEC, int PER>
+// PER > 0: the row in registers, PER * VEC * blockDim >= cols.  PER = 0: any length, read twice.  ANY (with PER > 0): inputs at any address and
+// of any length.
+template <typename T, int KIND, int VEC, int PER, bool ANY = false>
 __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
   pdl_launch_dependents();
   pdl_wait();
@@ -169,7 +272,8 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
     for (int i = 0; i < PER; ++i) {
       const int c = (i * blockDim.x + threadIdx.x) * VEC;
       if (c < p.cols) {
-        rq_load<T, KIND, VEC>(p, x, res, c, v[i], s[i]);
+        if constexpr (ANY) rq_load_any<T, KIND, VEC>(p, row, x, res, c, v[i], s[i]);
+        else rq_load<T, KIND, VEC>(p, x, res, c, v[i], s[i]);
       } else {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[i][e] = s[i][e] = 0.f;
@@ -179,7 +283,11 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
     for (int i = 0; i < PER; ++i) {
       rq_account<KIND, VEC>(v[i], s[i], sum, most);
       const int c = (i * blockDim.x + threadIdx.x) * VEC;
-      if (KIND == RQ_NORM && res != nullptr && c < p.cols) store_vec<T, VEC>(res + c, s[i]);
+      if constexpr (KIND == RQ_NORM && ANY) {
+        if (res != nullptr) rq_store_any<T, VEC>(res + c, p.cols - c, s[i]);  // (whole warps)
+      } else {
+        if (KIND == RQ_NORM && res != nullptr && c < p.cols) store_vec<T, VEC>(res + c, s[i]);
+      }
     }
   } else {
     for (int c = threadIdx.x * VEC; c < p.cols; c += blockDim.x * VEC) {
@@ -193,7 +301,7 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = (i * blockDim.x + threadIdx.x) * VEC;
-      if (c < p.cols) rq_store<VEC>(r, out + c, v[i]);
+      if (c < p.cols) rq_store<VEC>(r, out + c, v[i], ANY ? p.cols - c : VEC);
     }
   } else {
     for (int c = threadIdx.x * VEC; c < p.cols; c += blockDim.x * VEC) {
@@ -278,7 +386,7 @@ static int g_rq_sms = 0;
 // 53.7 and 75.7, 2,048 x 16,384 plain 18.8 and 25.9, 1,000 11.7 and 14.3, 300 6.6 and 6.1; 2,048 x 8,192 plain 11.8 and 12.2, gated 19.6
 // and 19.4.  A norm reads its weight beside the rows and is never faster there (2,048 x 4,096 14.2 and 13.0).
 template <typename T, int KIND>
-static bool rq_try_stream(RqParams p, int rows, cudaStream_t st, int* code) {
+static bool rq_try_stream(const RqParams& p, int rows, cudaStream_t st, int* code) {
   constexpr int VEC = 16 / (int)sizeof(T);
   if (g_rq_sms == 0) {
     int dev = 0;
@@ -299,15 +407,15 @@ static bool rq_try_stream(RqParams p, int rows, cudaStream_t st, int* code) {
   if (per_sm > 1088 / threads) per_sm = 1088 / threads;  // (60 registers a thread)
   if (per_sm < 1) per_sm = 1;
   const int most = per_sm * g_rq_sms, each = (rows + most - 1) / most;  // (every block the same number of rows, or one less)
-  p.rows = rows;
   *code = ullm_launch_kernel(rows_int8_stream<T, KIND>, dim3((rows + each - 1) / each), dim3(threads), smem, st, p);
   return true;
 }
 
 // Groups of a thread.  One, where a row's groups are threads enough: 2,048 x 4,096 normed 13.0 us, with two 15.2; rows as they are are
 // less work and take two from 256 groups on (2,048 x 4,096 6.7 for 8.0, 8 x 8,192 1.61 for 1.69).  Element by element many rows take two
-// from 384 on and four from 768 (1,000 x 2,043 normed 9.7, with two 11.7, with eight 13.3; 1,000 x 531 3.3, with one 4.8).
-template <typename T, int KIND, int VEC>
+// from 384 on (1,000 x 531 normed 3.3, with one 4.8) and four from 768 (8-bit rows anywhere: 1,000 x 2,043 9.7, with two 11.7, with eight
+// 13.3).
+template <typename T, int KIND, int VEC, bool ANY = false>
 static int rq_launch_vec(const RqParams& p, int rows, cudaStream_t st) {
   const int groups = (p.cols + VEC - 1) / VEC;
   auto go = [&](auto kernel, int per) {
@@ -318,9 +426,9 @@ static int rq_launch_vec(const RqParams& p, int rows, cudaStream_t st) {
   if constexpr (VEC == 1) {
     if (groups > 4096 && groups <= 8192) return go(rows_int8_kernel<T, KIND, VEC, 8>, 8);
   }
-  if (groups <= 1024 && least < 2) return go(rows_int8_kernel<T, KIND, VEC, 1>, 1);
-  if (groups <= 2048 && least < 3) return go(rows_int8_kernel<T, KIND, VEC, 2>, 2);
-  if (groups <= 4096) return go(rows_int8_kernel<T, KIND, VEC, 4>, 4);
+  if (groups <= 1024 && least < 2) return go(rows_int8_kernel<T, KIND, VEC, 1, ANY>, 1);
+  if (groups <= 2048 && least < 3) return go(rows_int8_kernel<T, KIND, VEC, 2, ANY>, 2);
+  if (groups <= 4096) return go(rows_int8_kernel<T, KIND, VEC, 4, ANY>, 4);
   return go(rows_int8_kernel<T, KIND, VEC, 0>, 4);
 }
 
@@ -334,15 +442,25 @@ static int rq_launch(const RqParams& p, int rows, cudaStream_t st) {
   if constexpr (KIND != RQ_NORM) {
     if (wide && rq_try_stream<T, KIND>(p, rows, st, &code)) return code;
   }
-  return wide ? rq_launch_vec<T, KIND, V>(p, rows, st) : rq_launch_vec<T, KIND, 1>(p, rows, st);
+  if (wide) return rq_launch_vec<T, KIND, V>(p, rows, st);
+  // Pieces that are shifted into place cost little rows a longer way (the ends' elements come one by one) and many rows less work.  us so
+  // and element by element, normed, bfloat16: 1 x 4,091 2.8 and 2.9, 1 x 1,003 2.7 and 1.8; 64 x 2,043 3.0 and 3.0, 300 x 1,003 3.2 and 3.5,
+  // 1,000 x 531 5.0 and 3.3, 2,048 x 531 5.8 and 6.4; 2,048 x 4,091 22.8 and 34.4.  Plain 2,048 x 8,001 16.4 and 42.6, gated 2,048 x 9,001
+  // 35.6 and 67.2.
+  const long long n = (long long)rows * p.cols;
+  const bool many = p.cols >= 4000 || (p.cols >= 1000 && n >= 1 << 17) || (p.cols >= 500 && n >= 1 << 20);
+  const bool borders = (uintptr_t)p.weight % 16 == 0 && (uintptr_t)p.out % V == 0 && p.out_stride % V == 0;
+  if (many && borders && p.cols <= 4096 * V) return rq_launch_vec<T, KIND, V, true>(p, rows, st);
+  return rq_launch_vec<T, KIND, 1>(p, rows, st);
 }
 
 template <int KIND>
-static int rq_run(int dtype, const RqParams& p, int rows, void* stream) {
+static int rq_run(int dtype, RqParams p, int rows, void* stream) {
   if (rows < 0 || p.cols <= 0 || p.cols > (1 << 28) || p.out_stride < p.cols || p.x_stride < p.cols) return ULLM_ERR_BAD_SIZE;
   if (dtype != ULLM_DTYPE_F32 && dtype != ULLM_DTYPE_BF16 && dtype != ULLM_DTYPE_F16) return ULLM_ERR_BAD_DTYPE;
   if (rows == 0) return ULLM_OK;
   cudaStream_t st = (cudaStream_t)stream;
+  p.rows = rows;
   if (dtype == ULLM_DTYPE_F32) return rq_launch<float, KIND>(p, rows, st);
   if (dtype == ULLM_DTYPE_BF16) return rq_launch<__nv_bfloat16, KIND>(p, rows, st);
   return rq_launch<__half, KIND>(p, rows, st);
