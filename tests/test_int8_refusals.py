@@ -34,7 +34,7 @@ def test_launchers(lib):
     assert lib.ullm_add_rmsnorm_int8(5, None, None, None, None, 8, None, 4, 8, 1e-6, None, None) == BAD_DTYPE
     assert lib.ullm_add_rmsnorm_int8(1, None, None, None, None, 4, None, 4, 8, 1e-6, None, None) == BAD_SIZE
     for dtype, M, N, k, xs, ws, want in ((0, 4, 8, 0, 16, 16, BAD_SIZE), (0, 4, 8, 131072, 131072, 131072, BAD_SIZE),
-                                         (0, 4, 0, 16, 16, 16, BAD_SIZE), (0, -1, 8, 16, 16, 16, BAD_SIZE), (0, 4, 8, 16, 15, 16, BAD_SIZE),
+                                         (0, 4, 0, 16, 16, 16, BAD_SIZE), (0, (1 << 30) + 1, 8, 16, 16, 16, BAD_SIZE), (0, 4, (1 << 30) + 1, 16, 16, 16, BAD_SIZE), (0, -1, 8, 16, 16, 16, BAD_SIZE), (0, 4, 8, 16, 15, 16, BAD_SIZE),
                                          (0, 4, 8, 16, 16, 8, BAD_SIZE), (7, 4, 8, 16, 16, 16, BAD_DTYPE), (1, 0, 8, 16, 16, 16, 0)):
         assert lib.ullm_linear_int8(dtype, None, xs, None, None, ws, None, None, None, M, N, k, None, None) == want
 

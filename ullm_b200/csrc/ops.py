@@ -890,7 +890,7 @@ class Kernels:
     def linear_int8(self, x, x_scales, weight, w_scales, out, bias=None):
         """out[t, n] = (sum_k x[t, k] weight[n, k]) * x_scales[t] * w_scales[n] (+ bias[n]): x int8 [T, K], weight int8 [N, K], scales
         float32 [T] and [N], out [T, N] float32, bfloat16 or float16, bias [N] of out's type.  The sums are whole numbers and exact
-        (K up to 131,071), the result is formed in 32-bit and rounded once (csrc/linear_int8.cu)."""
+        (K up to 131,071; T and N up to 2^30), the result is formed in 32-bit and rounded once (csrc/linear_int8.cu)."""
         if self._unwatched() and _at_once.linear_int8(self.lib.ullm_linear_int8, x, x_scales, weight, w_scales, out, bias,
                                                       self.status) == 0:
             self.launches += 1
