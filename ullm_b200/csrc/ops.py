@@ -807,7 +807,8 @@ class Kernels:
 
     # -- 8-bit rows and their products ---------------------------------------
     # An 8-bit row q (int8) with the scale s (float32) stands for the values q * s: s = max|y| / 127 of the row y that it was made of, q
-    # the whole numbers nearest to y / s, ties to even.  A row of zeros has the scale 0; a row that holds an infinity or a NaN has the
+    # the whole numbers nearest to 127 y / max|y|, ties to even (where y is formed in 32 bits first, normed or gated, a tie is an
+    # accident of that rounding and may go either way).  A row of zeros has the scale 0; a row that holds an infinity or a NaN has the
     # scale NaN (and zeros), so that all that is made of it is NaN.  Rows may lie apart (`int8_rows`): the product takes rows on borders
     # of 16 bytes to the tensor cores and any others to a plain kernel that is ten times slower.
     #

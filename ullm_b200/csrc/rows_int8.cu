@@ -10,11 +10,18 @@
 // The norm needs one pass: y = rstd * (s w) with rstd the same for the whole row, so max|y| = rstd max|s w| and the whole numbers are
 // those of s w, which the statistics do not enter.  Sum of squares and maximum come out of the same reduction (one barrier).
 //
-// Rounding: s w * (127 / max) + 1.5 * 2^23 in one fused multiply-add leaves the nearest whole number, ties to even, in the sum's low
-// bits (two's complement); |s w * (127 / max)| is at most 127 (1 + 2^-23), which is 127 again.  A row whose maximum is below 2^-90 is
-// multiplied by 2^100 first, so that 127 / max stays finite.  A row of zeros gets the scale 0 (the norm's formula: NaN where eps is 0
-// too).  A row that holds an infinity or a NaN has no scale: it gets the scale NaN and zeros, so that everything made of it is NaN and
-// the other rows are untouched.  (Between threads the maximum is taken of bit patterns, in whose order infinities and then NaN come last.)
+// Rounding: s w * (127 / max) + 1.5 * 2^23 in one fused multiply-add leaves the nearest whole number in the sum's low bits (two's
+// complement); |s w * (127 / max)| is at most 127 (1 + 2^-23), which is 127 again.  Ties of rows as they are go to even although the
+// quotient 127 / max is rounded: v is halfway between two whole numbers where 254 v = odd * max, an odd number below 254, so that 127
+// divides that odd number or the significand of max.  The first is v = max / 2, which stands for 63.5 (of 16-bit rows one element in some
+// hundred): the quotient is rounded up, and it becomes 64.  Rows of the second kind, one in 127 (bfloat16: none whose quotient is not
+// exact), have an exact max / 127, by which the quotient's product is corrected (`rq_quotient`).  All other elements of 16-bit rows are
+// further than 2^-19 of their value from a middle, further than the quotient's 2^-23; of 32-bit rows, and of rows that are formed here and
+// rounded themselves, what lies nearer to one may go to either side.  A row whose maximum is below 2^-90 is multiplied by 2^100 first, so
+// that 127 / max stays finite.
+// A row of zeros gets the scale 0 (the norm's formula: NaN where eps is 0 too).  A row that holds an infinity or a NaN has no scale: it
+// gets the scale NaN and zeros, so that everything made of it is NaN and the other rows are untouched.  (Between threads the maximum is
+// taken of bit patterns, in whose order infinities and then NaN come last.)
 //
 // The work is bound by memory.  Two forms:
 //   rows_int8_kernel   a block takes one row and holds it in registers between the reduction and the store (PER groups of VEC
@@ -23,6 +30,8 @@
 //                      element.
 //   rows_int8_stream   blocks that stay and take one row after the other, the next rows on their way into shared memory (bulk copies)
 //                      while one is worked on.  Many rows.
+#include <type_traits>
+
 #include "tcgen05_util.cuh"
 
 #define RQ_PLAIN 0
@@ -82,13 +91,26 @@ struct RqRow {
   float mul;        // out = round(v * mul)
   uint32_t keep;    // all ones, or 0 for a row that is not finite
   bool tiny;        // ... of v * 2^100
-  float most;
+  float step;       // max / 127 (of v * 2^100) where that is exact and `mul` is not, else 0
+  float most;       // the row's largest
 };
+template <typename T, int KIND>
+constexpr bool rq_ties = KIND == RQ_PLAIN && !std::is_same<T, __nv_bfloat16>::value;  // whether `step` is asked for at all
+template <typename T, int KIND>
 __device__ __forceinline__ RqRow rq_row(uint32_t top) {
   RqRow r;
   const float most = r.most = __uint_as_float(top);
   r.tiny = most < 8.077935669463161e-28f;  // 2^-90
-  r.mul = top == 0u ? 0.f : 127.f / (r.tiny ? most * 1.2676506002282294e30f : most);
+  const float top_of = r.tiny ? most * 1.2676506002282294e30f : most;
+  float mul = 127.f / top_of;
+  const float rest = fmaf(mul, top_of, -127.f);
+  if (KIND != RQ_ACT && rest < 0.f) mul = __uint_as_float(__float_as_uint(mul) + 1);
+  r.mul = top == 0u ? 0.f : mul;
+  r.step = 0.f;
+  if constexpr (rq_ties<T, KIND>) {
+    const float step = top_of / 127.f;
+    if (rest != 0.f && fmaf(step, 127.f, -top_of) == 0.f) r.step = step;
+  }
   r.keep = top < 0x7f800000u ? 0xffffffffu : 0u;
   return r;
 }
@@ -225,10 +247,19 @@ __device__ __forceinline__ void rq_account(const float (&v)[VEC], const float (&
     if (KIND == RQ_NORM) sum = fmaf(s[i], s[i], sum);
   }
 }
-template <int VEC>
+// v / step where `step` is exact: a product with the rounded reciprocal and what it left, so that a quotient of 24 bits comes out as it is
+__device__ __forceinline__ float rq_quotient(float v, float mul, float step) {
+  const float t = v * mul;
+  return fmaf(fmaf(-t, step, v), mul, t);
+}
+template <bool TIES, int VEC>
 __device__ __forceinline__ void rq_store(const RqRow& r, signed char* out, const float (&v)[VEC], int left = VEC) {
   uint32_t q[VEC];
-  if (r.tiny) {
+  if (TIES && r.step != 0.f) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      q[i] = __float_as_uint(rq_quotient(r.tiny ? v[i] * 1.2676506002282294e30f : v[i], r.mul, r.step) + 12582912.f);
+  } else if (r.tiny) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) q[i] = __float_as_uint(fmaf(v[i] * 1.2676506002282294e30f, r.mul, 12582912.f));
   } else {
@@ -295,19 +326,19 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
       rq_account<KIND, VEC>(v[0], s[0], sum, most);
     }
   }
-  const RqRow r = rq_row(rq_reduce(sum, most, KIND == RQ_NORM));
+  const RqRow r = rq_row<T, KIND>(rq_reduce(sum, most, KIND == RQ_NORM));
   if (threadIdx.x == 0) p.scales[row] = rq_scale(r, KIND == RQ_NORM ? rsqrtf(sum / (float)p.cols + p.eps) : 1.f);
   if constexpr (PER > 0) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = (i * blockDim.x + threadIdx.x) * VEC;
-      if (c < p.cols) rq_store<VEC>(r, out + c, v[i], ANY ? p.cols - c : VEC);
+      if (c < p.cols) rq_store<rq_ties<T, KIND>, VEC>(r, out + c, v[i], ANY ? p.cols - c : VEC);
     }
   } else {
     for (int c = threadIdx.x * VEC; c < p.cols; c += blockDim.x * VEC) {
       rq_load<T, KIND, VEC>(p, x, res, c, v[0], s[0]);
       if (KIND == RQ_NORM && res != nullptr) store_vec<T, VEC>(res + c, s[0]);
-      rq_store<VEC>(r, out + c, v[0]);
+      rq_store<rq_ties<T, KIND>, VEC>(r, out + c, v[0]);
     }
   }
 }
@@ -361,7 +392,7 @@ __global__ void __launch_bounds__(1024) rows_int8_stream(const RqParams p) {
         rq_account<KIND, VEC>(v[i], s, sum, most);
       }
     }
-    const RqRow r = rq_row(rq_reduce(sum, most, false, turn));
+    const RqRow r = rq_row<T, KIND>(rq_reduce(sum, most, false, turn));
     if (threadIdx.x == 0) {
       const long long next = row + (long long)RQ_SLOTS * gridDim.x;
       if (ok && next < p.rows) ask(next, slot);
@@ -371,7 +402,7 @@ __global__ void __launch_bounds__(1024) rows_int8_stream(const RqParams p) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = (i * blockDim.x + threadIdx.x) * VEC;
-      if (c < p.cols) rq_store<VEC>(r, out + c, v[i]);
+      if (c < p.cols) rq_store<rq_ties<T, KIND>, VEC>(r, out + c, v[i]);
     }
     turn ^= 1;
     if (++slot == RQ_SLOTS) slot = 0, parity ^= 1;
