@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from conftest import device
+from plain_int8 import check_rows, gated
 from test_gpu_kernels import K
 
 pytestmark = [pytest.mark.gpu, pytest.mark.needs_cuda]
@@ -95,3 +96,30 @@ def test_a_half_of_the_largest_is_64():
         q, scales = torch.empty(count, 64, dtype=torch.int8, device=device()), torch.empty(count, device=device())
         K().quantize_rows_int8(x, q, scales)
         assert (q[:, 0] == 127).all() and (q[:, 1:] == -64).all()
+
+
+# rows in registers (one, two and four groups a thread), of any length, element by element, read twice, and blocks that stay
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", [0, 1])
+@pytest.mark.parametrize("rows,cols", [(4, 5), (9, 1024), (9, 9000), (9, 20000), (4, 40000), (700, 4101), (9, 1003), (600, 16384)])
+def test_gates_far_below_zero(rows, cols, act, dtype):
+    """Gates whose activation is below 2^-126: rows of these alone, beside ups that make more of it (2^80; float16 has none such), and beside
+    ordinary ones."""
+    g = torch.Generator(device=device()).manual_seed(cols)
+    x = torch.randn(rows, 2 * cols, generator=g, device=device())
+    lowest = torch.rand(rows, cols, generator=g, device=device())
+    x[:, :cols] = -85 - 60 * lowest if act == 0 else -9.7 - 1.5 * lowest
+    x[:, cols:] *= 1.0 if dtype == torch.float16 else 2.0 ** 80
+    x[1] = torch.randn(2 * cols, generator=g, device=device())
+    x[1, 0], x[1, cols] = -100.0, 1.0  # (nothing that counts)
+    x[2, cols - 1] = 30.0 if act == 0 else 9.5  # (and the rest of the row is nothing beside it)
+    x[3] = 0.0
+    x = x.to(dtype)
+    q, scales = K().int8_rows(rows, cols), torch.empty(rows, device=device())
+    K().act_mul_int8(x, q, scales, act)
+    y, z = gated(x, act)
+    rel = 2.0 ** -22 * (z.abs() + 3)
+    fine = y.abs().amax(1) > 2.0 ** -125  # (32-bit numbers below 2^-126 have fewer bits)
+    fine[3] = True
+    check_rows(q[fine], scales[fine], y[fine], rel[fine], float(rel.max()))
+    assert scales[3] == 0 and not q[3].any() and fine[:3].sum() >= (2 if dtype == torch.float16 else 3)

@@ -868,7 +868,8 @@ class Kernels:
 
     def act_mul_int8(self, gate_up, out, scales, act: int = 0):
         """`act_mul` with its result in 8 bits: out (int8 [T, I]), scales (float32 [T]) <- the rows act(gate) * up of gate_up
-        [T, 2 I] = [gate | up], in 32-bit up to there (act 0 silu, 1 gelu_tanh)."""
+        [T, 2 I] = [gate | up], in 32-bit up to there (act 0 silu, 1 gelu_tanh).  An activation below 2^-126 counts as zero beside an
+        up above 2^91 (the only place where more than half a step could be made of it)."""
         if self._unwatched() and _at_once.act_mul_int8(self.lib.ullm_act_mul_int8, gate_up, out, scales, act, self.status) == 0:
             self.launches += 1
             return out

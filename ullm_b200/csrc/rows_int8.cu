@@ -53,21 +53,48 @@ struct RqParams {
 };
 
 // A gate's activation g / (1 + e^-z), z = g (silu) or 2 sqrt(2 / pi) (g + 0.044715 g^3) (gelu_tanh, since (1 + tanh v) / 2 =
-// 1 / (1 + e^-2v)), in six instructions without a branch: -z log2 e, 2^x, one more, the reciprocal, two products with up's.  A
-// denominator beyond 2^126 has the reciprocal 0, where the true value is below 2^-119.  Off by 2^-22 (|z| + 2.25) of its value: a step
-// or two each, and what the roundings of the exponent make of it.
-__device__ __forceinline__ float rq_gate(float g, int act) {
-  const float z = act == 0 ? g * -1.4426950408889634f : g * fmaf(g * g, -0.10294324f, -2.3022082f);
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+// 1 / (1 + e^-2v)), in six instructions without a branch: t = -z log2 e, 2^t, one more, the reciprocal, two products with up's.  Off by
+// 2^-22 (|z| + 2.25) of its value: a step or two each, and what the roundings of the exponent make of it.  Where 1 + 2^t passes 2^126 the
+// reciprocal is 0, for an activation of up to 2^-119; `rq_act_again` has the rows in which that shows.
+__device__ __forceinline__ float rq_exponent(float g, int act) {
+  return act == 0 ? g * -1.4426950408889634f : g * fmaf(g * g, -0.10294324f, -2.3022082f);
+}
+__device__ __forceinline__ float rq_exp2(float t) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return e;
+}
+__device__ __forceinline__ float rq_gate(float g, float t) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + rq_exp2(t)));
   return g * r;
 }
-// the larger magnitude, NaN where either is
+// act(g) * up for any exponent: where 1 is nothing beside 2^t, both factors take half of it (off by 2^-22 (|z| + 3))
+__device__ __forceinline__ float rq_gate_times(float g, float up, int act) {
+  const float t = rq_exponent(g, act), half = rq_exp2(-0.5f * t);
+  return t > 125.f ? (g * half) * (up * half) : rq_gate(g, t) * up;
+}
+// the largest magnitude, NaN where one is
 __device__ __forceinline__ float rq_max(float top, float v) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(v)));
   return r;
+}
+__device__ __forceinline__ float rq_max(float top, float v, float u) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(top), "f"(fabsf(v)), "f"(fabsf(u)));
+  return r;
+}
+// the larger of top and the VEC magnitudes
+template <int VEC>
+__device__ __forceinline__ float rq_most(float top, const float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    top = rq_max(top, v[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) top = rq_max(top, v[i], v[i + 1]);
+  }
+  return top;
 }
 
 // (sum, bits of the largest magnitude) over the block, the same in every thread; the order of additions depends on blockDim alone
@@ -193,7 +220,7 @@ __device__ __forceinline__ void rq_load(const RqParams& p, const T* x, const T* 
   if constexpr (KIND == RQ_ACT) {
     load_vec<T, VEC>(x + p.cols + c, s);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = rq_gate(v[i], p.act) * s[i];
+    for (int i = 0; i < VEC; ++i) v[i] = rq_gate(v[i], rq_exponent(v[i], p.act)) * s[i];
   }
   if constexpr (KIND == RQ_NORM) {
     if (res != nullptr) {
@@ -218,7 +245,7 @@ __device__ __forceinline__ void rq_load_any(const RqParams& p, long long row, co
   if constexpr (KIND == RQ_ACT) {
     rq_read<T, VEC>(x + p.cols + c, begin + p.cols, end - begin - p.cols, left, s);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = rq_gate(v[i], p.act) * s[i];
+    for (int i = 0; i < VEC; ++i) v[i] = rq_gate(v[i], rq_exponent(v[i], p.act)) * s[i];
   }
   if constexpr (KIND == RQ_NORM) {
     if (res != nullptr) {
@@ -241,10 +268,10 @@ __device__ __forceinline__ void rq_load_any(const RqParams& p, long long row, co
 }
 template <int KIND, int VEC>
 __device__ __forceinline__ void rq_account(const float (&v)[VEC], const float (&s)[VEC], float& sum, float& top) {
+  top = rq_most<VEC>(top, v);
+  if constexpr (KIND == RQ_NORM) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    top = rq_max(top, v[i]);
-    if (KIND == RQ_NORM) sum = fmaf(s[i], s[i], sum);
+    for (int i = 0; i < VEC; ++i) sum = fmaf(s[i], s[i], sum);
   }
 }
 // v / step where `step` is exact: a product with the rounded reciprocal and what it left, so that a quotient of 24 bits comes out as it is
@@ -284,6 +311,25 @@ __device__ __forceinline__ void rq_store(const RqRow& r, signed char* out, const
     if (i < left) out[i] = (signed char)(q[i] & r.keep & 0xff);
 }
 
+// A gated row in which the elements beyond the fast gate may count, by the whole block, two reads of the row x [gate | up].  They are up to
+// 2^-119 |up| each: below half a step, and so nothing, where the row's largest is not below 2^-20 and no up above 2^91.  (Looking for
+// such ups would cost every row: 16 x 12,288 2.64 us and 2.80.  Beside one, a gate that far below zero counts as zero.)
+template <typename T>
+__device__ __noinline__ void rq_act_again(const T* x, signed char* out, float* scale, int cols, int act) {
+  float none = 0.f, most = 0.f;
+  for (int c = threadIdx.x; c < cols; c += blockDim.x) most = rq_max(most, rq_gate_times(to_f32(x[c]), to_f32(x[cols + c]), act));
+  const RqRow r = rq_row<T, RQ_ACT>(rq_reduce(none, most, false));
+  if (threadIdx.x == 0) *scale = rq_scale(r, 1.f);
+  for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+    const float v[1] = {rq_gate_times(to_f32(x[c]), to_f32(x[cols + c]), act)};
+    rq_store<false, 1>(r, out + c, v);
+  }
+}
+template <int KIND>
+__device__ __forceinline__ bool rq_is_far(uint32_t top) {
+  return KIND == RQ_ACT && top < 0x35800000u;  // 2^-20
+}
+
 // PER > 0: the row in registers, PER * VEC * blockDim >= cols.  PER = 0: any length, read twice.  ANY (with PER > 0): inputs at any address and
 // of any length.
 template <typename T, int KIND, int VEC, int PER, bool ANY = false>
@@ -296,8 +342,7 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
   signed char* out = p.out + row * p.out_stride;
   constexpr int P = PER > 0 ? PER : 1;
   float v[P][VEC], s[P][VEC];
-  float sum = 0.f;
-  float most = 0.f;
+  float sum = 0.f, most = 0.f;
   if constexpr (PER > 0) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -326,7 +371,11 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
       rq_account<KIND, VEC>(v[0], s[0], sum, most);
     }
   }
-  const RqRow r = rq_row<T, KIND>(rq_reduce(sum, most, KIND == RQ_NORM));
+  const uint32_t top = rq_reduce(sum, most, KIND == RQ_NORM);
+  if constexpr (KIND == RQ_ACT) {
+    if (rq_is_far<KIND>(top)) return rq_act_again(x, out, p.scales + row, p.cols, p.act);
+  }
+  const RqRow r = rq_row<T, KIND>(top);
   if (threadIdx.x == 0) p.scales[row] = rq_scale(r, KIND == RQ_NORM ? rsqrtf(sum / (float)p.cols + p.eps) : 1.f);
   if constexpr (PER > 0) {
 #pragma unroll
@@ -392,17 +441,22 @@ __global__ void __launch_bounds__(1024) rows_int8_stream(const RqParams p) {
         rq_account<KIND, VEC>(v[i], s, sum, most);
       }
     }
-    const RqRow r = rq_row<T, KIND>(rq_reduce(sum, most, false, turn));
+    const uint32_t top = rq_reduce(sum, most, false, turn);
+    const RqRow r = rq_row<T, KIND>(top);
     if (threadIdx.x == 0) {
       const long long next = row + (long long)RQ_SLOTS * gridDim.x;
       if (ok && next < p.rows) ask(next, slot);
       p.scales[row] = rq_scale(r, 1.f);
     }
     signed char* out = p.out + row * p.out_stride;
+    if (KIND == RQ_ACT && rq_is_far<KIND>(top)) {
+      rq_act_again(reinterpret_cast<const T*>(p.x) + row * p.x_stride, out, p.scales + row, p.cols, p.act);
+    } else {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * VEC;
-      if (c < p.cols) rq_store<rq_ties<T, KIND>, VEC>(r, out + c, v[i]);
+      for (int i = 0; i < PER; ++i) {
+        const int c = (i * blockDim.x + threadIdx.x) * VEC;
+        if (c < p.cols) rq_store<rq_ties<T, KIND>, VEC>(r, out + c, v[i]);
+      }
     }
     turn ^= 1;
     if (++slot == RQ_SLOTS) slot = 0, parity ^= 1;
