@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from conftest import device
-from plain_int8 import check_rows, gated
+from plain_int8 import check_rows, gated, normed
 from test_gpu_kernels import K
 
 pytestmark = [pytest.mark.gpu, pytest.mark.needs_cuda]
@@ -123,3 +123,30 @@ def test_gates_far_below_zero(rows, cols, act, dtype):
     fine[3] = True
     check_rows(q[fine], scales[fine], y[fine], rel[fine], float(rel.max()))
     assert scales[3] == 0 and not q[3].any() and fine[:3].sum() >= (2 if dtype == torch.float16 else 3)
+
+
+# rows in registers (one, two and four groups a thread), of any length, element by element, read twice
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("with_residual", [True, False])
+@pytest.mark.parametrize("cols", [5, 1024, 4096, 9000, 16384, 20000, 33000, 40000, 4101, 1003])
+def test_norms_whose_squares_pass_32_bits(cols, with_residual, dtype):
+    """Rows of every size with an eps that counts and with none, and rows that hold one element of that size."""
+    g = torch.Generator(device=device()).manual_seed(cols)
+    sizes = torch.tensor([-110, -80, -64, -63, -50, -40, -38, -10, 0, 40, 45, 50, 55, 60, 63, 64, 65, 80, 100, 110, 122], device=device())
+    sizes = sizes.repeat_interleave(2).double()[:, None]
+    x = torch.randn(len(sizes), cols, generator=g, device=device(), dtype=torch.float64)
+    one = torch.where(torch.arange(cols, device=device()) == cols - 2, 2.0 ** sizes[1::2], 1.0)
+    x[::2] *= 2.0 ** sizes[::2]
+    x[1::2] *= one
+    x = x.to(dtype)
+    residual = (x.roll(1, 1) * 0.5) if with_residual else None
+    weight = 1 + 0.3 * torch.randn(cols, generator=g, device=device())
+    for eps in (1e-6, 0.0, 2.0 ** -60):
+        res = residual.clone() if with_residual else None
+        q, scales = K().int8_rows(len(x), cols), torch.empty(len(x), device=device())
+        K().add_rmsnorm_int8(x, res, weight, eps, q, scales)
+        # as for rows of ordinary size (an element: the sum and the weight's product; a scale: besides, half of the sum of squares' error),
+        # and squares that are below 2^-126 beside an eps above 2^-73: below 2^-40 of it
+        check_rows(q, scales, normed(x, residual, weight, eps), 2.0 ** -23, 2.0 ** -24 * ((cols / 1024 + 40) / 2 + 10))
+        if with_residual:
+            assert torch.equal(res, (x.float() + residual.float()).to(dtype))

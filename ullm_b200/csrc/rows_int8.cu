@@ -8,7 +8,8 @@
 //   s * rsqrt(mean(s^2) + eps) * w         (RMSNorm) with s = x (+ residual), residual <- round(s)
 //
 // The norm needs one pass: y = rstd * (s w) with rstd the same for the whole row, so max|y| = rstd max|s w| and the whole numbers are
-// those of s w, which the statistics do not enter.  Sum of squares and maximum come out of the same reduction (one barrier).
+// those of s w, which the statistics do not enter.  Sum of squares and maximum come out of the same reduction (one barrier).  Rows of any
+// size have their scale (squares that 32 bits do not hold: RqSum) as long as s w is finite in 32 bits.
 //
 // Rounding: s w * (127 / max) + 1.5 * 2^23 in one fused multiply-add leaves the nearest whole number in the sum's low bits (two's
 // complement); |s w * (127 / max)| is at most 127 (1 + 2^-23), which is 127 again.  Ties of rows as they are go to even although the
@@ -141,8 +142,8 @@ __device__ __forceinline__ RqRow rq_row(uint32_t top) {
   r.keep = top < 0x7f800000u ? 0xffffffffu : 0u;
   return r;
 }
-__device__ __forceinline__ float rq_scale(const RqRow& r, float rstd) {
-  return r.keep ? rstd * r.most / 127.f : __uint_as_float(0x7fc00000u);
+__device__ __forceinline__ float rq_scale(const RqRow& r, float rstd = 1.f, float k = 1.f) {
+  return r.keep ? rstd * r.most * k / 127.f : __uint_as_float(0x7fc00000u);
 }
 
 // ---- rows that do not come in pieces of 16 bytes (ANY): a thread's group lies on its place of the row, wherever that is in memory ----
@@ -266,6 +267,40 @@ __device__ __forceinline__ void rq_load_any(const RqParams& p, long long row, co
     for (int i = 0; i < VEC; ++i) v[i] *= s[i];
   }
 }
+// A thread's sum of the squares of s * k.  Elements beyond 2^64 or so pass what 32 bits hold when they are squared, and where eps is next
+// to nothing the smallest fall below it: the sum begins with k = 1 (2^90 for such an eps) and goes on with the next smaller k where it
+// reaches 2^100.
+struct RqSum {
+  float sum = 0.f, k = 1.f;
+};
+#define RQ_SUM_LIMIT 1.2676506002282294e30f   // 2^100
+#define RQ_K_SMALL 1.2379400392853803e27f      // 2^90
+#define RQ_K_LARGE 8.271806125530277e-25f      // 2^-80
+__device__ __forceinline__ float rq_first_k(float eps) { return eps < 1.0587911840678754e-22f ? RQ_K_SMALL : 1.f; }  // 2^-73
+// whether a thread's plain sum of squares has to be formed so
+__device__ __forceinline__ bool rq_sum_again(float sum, float eps) { return !(sum < RQ_SUM_LIMIT) || rq_first_k(eps) != 1.f; }
+template <int VEC>
+__device__ __forceinline__ float rq_squares(const float (&s)[VEC], float sum, float k) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    const float t = s[i] * k;
+    sum = fmaf(t, t, sum);
+  }
+  return sum;
+}
+template <int VEC>
+__device__ __forceinline__ void rq_add(RqSum& a, const float (&s)[VEC]) {
+  float before = a.sum;
+  a.sum = rq_squares<VEC>(s, before, a.k);
+  if (!(a.sum < RQ_SUM_LIMIT) && a.k > 1.f) {
+    before = before / RQ_K_SMALL / RQ_K_SMALL, a.k = 1.f;
+    a.sum = rq_squares<VEC>(s, before, a.k);
+  }
+  if (!(a.sum < RQ_SUM_LIMIT) && a.k == 1.f) {
+    before = before * RQ_K_LARGE * RQ_K_LARGE, a.k = RQ_K_LARGE;
+    a.sum = rq_squares<VEC>(s, before, a.k);
+  }
+}
 template <int KIND, int VEC>
 __device__ __forceinline__ void rq_account(const float (&v)[VEC], const float (&s)[VEC], float& sum, float& top) {
   top = rq_most<VEC>(top, v);
@@ -273,6 +308,21 @@ __device__ __forceinline__ void rq_account(const float (&v)[VEC], const float (&
 #pragma unroll
     for (int i = 0; i < VEC; ++i) sum = fmaf(s[i], s[i], sum);
   }
+}
+// (bits of the largest magnitude, the sum of the squares of s * k) over the block; a.k <- that k
+template <int KIND>
+__device__ __forceinline__ uint32_t rq_join(const RqParams& p, RqSum& a, float most) {
+  if constexpr (KIND != RQ_NORM) return rq_reduce(a.sum, most, false);
+  float sum = a.k == rq_first_k(p.eps) ? a.sum : __uint_as_float(0x7f800000u);
+  const uint32_t top = rq_reduce(sum, most, true);
+  if (!(sum < 1.3292279957849159e36f)) {  // 2^120: some thread went on to a smaller k; the smallest is the one that all go by
+    float none = 0.f;
+    const float k = 1.f / __uint_as_float(rq_reduce(none, 1.f / a.k, false, 1));
+    sum = a.sum * (k / a.k) * (k / a.k), a.k = k;
+    rq_reduce(sum, 0.f, true);
+  }
+  a.sum = sum;
+  return top;
 }
 // v / step where `step` is exact: a product with the rounded reciprocal and what it left, so that a quotient of 24 bits comes out as it is
 __device__ __forceinline__ float rq_quotient(float v, float mul, float step) {
@@ -319,7 +369,7 @@ __device__ __noinline__ void rq_act_again(const T* x, signed char* out, float* s
   float none = 0.f, most = 0.f;
   for (int c = threadIdx.x; c < cols; c += blockDim.x) most = rq_max(most, rq_gate_times(to_f32(x[c]), to_f32(x[cols + c]), act));
   const RqRow r = rq_row<T, RQ_ACT>(rq_reduce(none, most, false));
-  if (threadIdx.x == 0) *scale = rq_scale(r, 1.f);
+  if (threadIdx.x == 0) *scale = rq_scale(r);
   for (int c = threadIdx.x; c < cols; c += blockDim.x) {
     const float v[1] = {rq_gate_times(to_f32(x[c]), to_f32(x[cols + c]), act)};
     rq_store<false, 1>(r, out + c, v);
@@ -342,7 +392,8 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
   signed char* out = p.out + row * p.out_stride;
   constexpr int P = PER > 0 ? PER : 1;
   float v[P][VEC], s[P][VEC];
-  float sum = 0.f, most = 0.f;
+  RqSum sum;
+  float most = 0.f;
   if constexpr (PER > 0) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -356,27 +407,42 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
       }
     }
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      rq_account<KIND, VEC>(v[i], s[i], sum, most);
-      const int c = (i * blockDim.x + threadIdx.x) * VEC;
-      if constexpr (KIND == RQ_NORM && ANY) {
-        if (res != nullptr) rq_store_any<T, VEC>(res + c, p.cols - c, s[i]);  // (whole warps)
-      } else {
-        if (KIND == RQ_NORM && res != nullptr && c < p.cols) store_vec<T, VEC>(res + c, s[i]);
+    for (int i = 0; i < PER; ++i) rq_account<KIND, VEC>(v[i], s[i], sum.sum, most);
+    if constexpr (KIND == RQ_NORM) {
+      if (rq_sum_again(sum.sum, p.eps)) {
+        sum.sum = 0.f, sum.k = rq_first_k(p.eps);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) rq_add<VEC>(sum, s[i]);
+      }
+      if (res != nullptr) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int c = (i * blockDim.x + threadIdx.x) * VEC;
+          if constexpr (ANY) rq_store_any<T, VEC>(res + c, p.cols - c, s[i]);  // (whole warps)
+          else if (c < p.cols) store_vec<T, VEC>(res + c, s[i]);
+        }
       }
     }
   } else {
     for (int c = threadIdx.x * VEC; c < p.cols; c += blockDim.x * VEC) {
       rq_load<T, KIND, VEC>(p, x, res, c, v[0], s[0]);
-      rq_account<KIND, VEC>(v[0], s[0], sum, most);
+      rq_account<KIND, VEC>(v[0], s[0], sum.sum, most);
+    }
+    if (KIND == RQ_NORM && rq_sum_again(sum.sum, p.eps)) {
+      sum.sum = 0.f, sum.k = rq_first_k(p.eps);
+      for (int c = threadIdx.x * VEC; c < p.cols; c += blockDim.x * VEC) {
+        rq_load<T, KIND, VEC>(p, x, res, c, v[0], s[0]);
+        rq_add<VEC>(sum, s[0]);
+      }
     }
   }
-  const uint32_t top = rq_reduce(sum, most, KIND == RQ_NORM);
+  const uint32_t top = rq_join<KIND>(p, sum, most);
   if constexpr (KIND == RQ_ACT) {
     if (rq_is_far<KIND>(top)) return rq_act_again(x, out, p.scales + row, p.cols, p.act);
   }
   const RqRow r = rq_row<T, KIND>(top);
-  if (threadIdx.x == 0) p.scales[row] = rq_scale(r, KIND == RQ_NORM ? rsqrtf(sum / (float)p.cols + p.eps) : 1.f);
+  if (threadIdx.x == 0)
+    p.scales[row] = KIND == RQ_NORM ? rq_scale(r, rsqrtf(sum.sum / (float)p.cols + p.eps * sum.k * sum.k), sum.k) : rq_scale(r);
   if constexpr (PER > 0) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -432,21 +498,21 @@ __global__ void __launch_bounds__(1024) rows_int8_stream(const RqParams p) {
     }
     const T* x = reinterpret_cast<const T*>(rq_ring + (size_t)slot * slot_bytes);
     float v[PER][VEC], s[VEC];
-    float sum = 0.f, most = 0.f;
+    float none = 0.f, most = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = (i * blockDim.x + threadIdx.x) * VEC;
       if (c < p.cols) {
         rq_load<T, KIND, VEC>(p, x, nullptr, c, v[i], s);
-        rq_account<KIND, VEC>(v[i], s, sum, most);
+        most = rq_most<VEC>(most, v[i]);
       }
     }
-    const uint32_t top = rq_reduce(sum, most, false, turn);
+    const uint32_t top = rq_reduce(none, most, false, turn);
     const RqRow r = rq_row<T, KIND>(top);
     if (threadIdx.x == 0) {
       const long long next = row + (long long)RQ_SLOTS * gridDim.x;
       if (ok && next < p.rows) ask(next, slot);
-      p.scales[row] = rq_scale(r, 1.f);
+      p.scales[row] = rq_scale(r);
     }
     signed char* out = p.out + row * p.out_stride;
     if (KIND == RQ_ACT && rq_is_far<KIND>(top)) {
