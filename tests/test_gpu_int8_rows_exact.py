@@ -150,3 +150,17 @@ def test_norms_whose_squares_pass_32_bits(cols, with_residual, dtype):
         check_rows(q, scales, normed(x, residual, weight, eps), 2.0 ** -23, 2.0 ** -24 * ((cols / 1024 + 40) / 2 + 10))
         if with_residual:
             assert torch.equal(res, (x.float() + residual.float()).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cols", [1 << 23, 5000001])
+def test_a_norm_of_millions_of_columns(cols, dtype):
+    """A thread's sum of thousands of squares: elements of one size, whose additions would all be rounded the same way, and others."""
+    x = torch.full((2, cols), 1.0078125, device=device()).to(dtype)
+    x[1] = torch.randn(cols, generator=torch.Generator(device=device()).manual_seed(1), device=device()).abs().to(dtype)
+    weight = torch.ones(cols, device=device())
+    q, scales = K().int8_rows(2, cols), torch.empty(2, device=device())
+    for size in (1.0, 2.0 ** 70):
+        K().add_rmsnorm_int8(x * size, None, weight, 1e-6, q, scales)
+        # half of the sum's error: eight of a thread's neighbouring elements, ten additions of the block, the sum rounded; the rest of a norm
+        check_rows(q, scales, normed(x * size, None, weight, 1e-6), 2.0 ** -23, 2.0 ** -24 * ((8 + 11) / 2 + 10))

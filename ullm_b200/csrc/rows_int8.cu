@@ -301,6 +301,10 @@ __device__ __forceinline__ void rq_add(RqSum& a, const float (&s)[VEC]) {
     a.sum = rq_squares<VEC>(s, before, a.k);
   }
 }
+__device__ __forceinline__ void rq_take(RqSum& a, double total, float k) {  // the same of a sum that is there
+  if (total * k * k >= RQ_SUM_LIMIT) k = total < RQ_SUM_LIMIT ? 1.f : RQ_K_LARGE;
+  a.sum = (float)(total * k * k), a.k = k;
+}
 template <int KIND, int VEC>
 __device__ __forceinline__ void rq_account(const float (&v)[VEC], const float (&s)[VEC], float& sum, float& top) {
   top = rq_most<VEC>(top, v);
@@ -424,16 +428,22 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
       }
     }
   } else {
+    double total = 0.0;  // (a thread's share has any number of elements: 2^18 of a row of 2^28)
     for (int c = threadIdx.x * VEC; c < p.cols; c += blockDim.x * VEC) {
       rq_load<T, KIND, VEC>(p, x, res, c, v[0], s[0]);
-      rq_account<KIND, VEC>(v[0], s[0], sum.sum, most);
+      float part = 0.f;
+      rq_account<KIND, VEC>(v[0], s[0], part, most);
+      total += part;
     }
+    sum.sum = (float)total;
     if (KIND == RQ_NORM && rq_sum_again(sum.sum, p.eps)) {
-      sum.sum = 0.f, sum.k = rq_first_k(p.eps);
+      total = 0.0;
       for (int c = threadIdx.x * VEC; c < p.cols; c += blockDim.x * VEC) {
         rq_load<T, KIND, VEC>(p, x, res, c, v[0], s[0]);
-        rq_add<VEC>(sum, s[0]);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) total += (double)s[0][i] * s[0][i];
       }
+      rq_take(sum, total, rq_first_k(p.eps));
     }
   }
   const uint32_t top = rq_join<KIND>(p, sum, most);
