@@ -175,8 +175,8 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
   constexpr int TMEM = NT < 32 ? 32 : NT;
   extern __shared__ unsigned char li_smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[LI_MAX_STAGES], empty_bar[LI_MAX_STAGES], acc_bar;
-  __shared__ uint32_t tmem_slot;
-  __shared__ int abort_flag;
+  __shared__ uint32_t tmem_slot, next_parity;
+  __shared__ int abort_flag, next_stage;  // (next_stage, next_parity: where the loads ended)
   __shared__ __align__(16) float xs_s[NT + 32];  // the tile's token scales
   unsigned char* ring = (unsigned char*)(((uintptr_t)li_smem_raw + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -229,6 +229,7 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
       }
       if (++s == p.stages) s = 0, parity ^= 1;
     }
+    if (lane == 0) next_stage = s, next_parity = parity;
   } else if (warp == 1) {
     constexpr uint32_t idesc = li_idesc(128, NT);
     const uint32_t lead = elect_one();
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
   __syncthreads();
   if (abort_flag && threadIdx.x == 0) {
     // a wait ran out: copies may still be on their way into the ring
-    for (int s = 0; s < p.stages && s < nst; ++s) mbar_wait(&full_bar[s], (((nst - 1 - s) / p.stages)) & 1);
+    for (int s = 0; s < p.stages; ++s) mbar_wait(&full_bar[s], ring_last_parity(s, next_stage, next_parity));
   }
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -407,7 +408,7 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
   extern __shared__ unsigned char li_smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_flag, go[2];
+  __shared__ int abort_flag, go[2], ended, other_ended;  // (where this block's loads ended; where the other's did, if it gave up)
   __shared__ __align__(16) float xs_s[2][BN];  // the token scales of a tile
   unsigned char* ring = (unsigned char*)(((uintptr_t)li_smem_raw + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -416,7 +417,7 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
   const long long tiles = (long long)t_tiles * ((p.N + 255) / 256);
 
   if (threadIdx.x == 0) {
-    abort_flag = 0;
+    abort_flag = 0, other_ended = -1;
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
@@ -467,10 +468,12 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
         if (++s == STAGES) s = 0, parity ^= 1;
       }
     }
+    if (lane == 0) ended = 2 * s + (int)parity;
     // (the commits that free the last stages arrive in both blocks: neither ends before)
     for (int i = 0; i < STAGES && ok; ++i) {
       if (!__all_sync(0xffffffffu, mbar_wait_addr(empty0 + s * 8, parity))) {
         if (lane == 0) ullm_report(p.status, ULLM_STATUS_TIMEOUT, 139, i);
+        abort_flag = 1;
         ok = false;
       }
       if (++s == STAGES) s = 0, parity ^= 1;
@@ -541,14 +544,22 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
     }
   }
   __syncthreads();
-  if (abort_flag && rank == 0 && threadIdx.x == 0) {
-    // a wait ran out: copies may still be on their way into either block's ring, whose bytes the leader's barriers count
-    const long long mine = tiles > cluster ? ((tiles - 1 - cluster) / clusters + 1) * p.k_blocks : 0;
-    for (int s = 0; s < STAGES && s < mine; ++s) mbar_wait(&full_bar[s], (uint32_t)((mine - 1 - s) / STAGES) & 1);
-  }
+  if (abort_flag && rank == 1 && threadIdx.x == 0)
+    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(li_rank_addr(lin_smem(&other_ended), 0)), "r"(ended) : "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   li_cluster_sync();  // nobody arrives at this block's barriers any more, or reads its ring
+  if (rank == 0 && threadIdx.x == 0 && (abort_flag || other_ended >= 0)) {
+    // A wait ran out: copies may still be on their way into either block's ring, whose bytes the leader's barriers count.  A stage that
+    // one block alone has filled never completes: the first such wait runs out, and the rest of that block's copies are there by then.
+    const long long all = tiles > cluster ? ((tiles - 1 - cluster) / clusters + 1) * p.k_blocks : 0;
+    const int planned = 2 * (int)(all % STAGES) + (int)((all / STAGES) & 1 ^ 1);
+    bool more = true;
+    for (int s = 0; s < STAGES && more; ++s) more = mbar_wait(&full_bar[s], ring_last_parity(s, ended >> 1, ended & 1));
+    const int other = other_ended >= 0 ? other_ended : planned;
+    for (int s = 0; s < STAGES && more; ++s) more = mbar_wait(&full_bar[s], ring_last_parity(s, other >> 1, other & 1));
+  }
+  __syncwarp();
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_d), "r"(COLUMNS) : "memory");
@@ -704,6 +715,8 @@ extern "C" int ullm_linear_int8_form(int M, int N, int K) {
   const LiForm f = li_choose(M, N, K);
   return f.pair ? -f.tile : 1000 * f.ksplit + f.tile;
 }
+
+extern "C" int ullm_ring_last_parity(int t, int s, int parity) { return (int)ring_last_parity(t, s, (uint32_t)parity); }
 
 // dtype: of out and bias.  Strides in bytes, at least K.
 extern "C" int ullm_linear_int8(int dtype, const void* x, long long x_stride, const void* x_scales, const void* w, long long w_stride,

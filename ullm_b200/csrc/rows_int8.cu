@@ -470,7 +470,8 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
 
 // One row after the other: two slots of shared memory hold a row's inputs each.  All of a block's threads have read a slot when they meet in
 // the reduction, so the copy of a later row into it is asked for right behind it.  Waits are bounded: one that runs out is recorded, and
-// the block goes on without waiting (its rows are then wrong, and the status word says so).
+// the thread goes on without waiting (the block's rows are then wrong, and the status word says so); no copy is asked for behind it, and
+// those that are on their way are waited for (bounded) at the end.
 #define RQ_SLOTS 2
 template <typename T, int KIND>
 __global__ void __launch_bounds__(1024) rows_int8_stream(const RqParams p) {
@@ -486,7 +487,9 @@ __global__ void __launch_bounds__(1024) rows_int8_stream(const RqParams p) {
   pdl_launch_dependents();
   __syncthreads();
   pdl_wait();
+  int asked = 0;  // (thread 0) copies so far, one slot after the other
   auto ask = [&](long long row, int slot) {
+    ++asked;
     const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_stride;
     mbar_expect_tx(&full_bar[slot], bytes);
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -538,7 +541,7 @@ __global__ void __launch_bounds__(1024) rows_int8_stream(const RqParams p) {
     if (++slot == RQ_SLOTS) slot = 0, parity ^= 1;
   }
   if (!ok && threadIdx.x == 0)  // copies may still be on their way into the slots
-    for (int s = 0; s < RQ_SLOTS; ++s) mbar_wait(&full_bar[s], s >= slot ? parity : parity ^ 1);
+    for (int s = 0; s < RQ_SLOTS; ++s) mbar_wait(&full_bar[s], ring_last_parity(s, asked % RQ_SLOTS, ((asked / RQ_SLOTS) & 1) ^ 1));
 }
 
 static int g_rq_sms = 0;

@@ -49,6 +49,9 @@ __device__ __forceinline__ bool mbar_wait_limited(uint64_t* bar, uint32_t parity
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
   return mbar_wait_limited(bar, parity, WAIT_LIMIT);
 }
+// A ring whose next copy goes to slot s, in a round in which an empty slot is waited for on `parity` (1 in the first round, 0 in the second,
+// and so on; a fresh barrier passes a wait on 1): the parity on which slot t's last copy is waited for, which passes at once where it has had none.
+__host__ __device__ __forceinline__ uint32_t ring_last_parity(int t, int s, uint32_t parity) { return t < s ? parity ^ 1u : parity; }
 __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
