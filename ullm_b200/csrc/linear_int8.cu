@@ -113,8 +113,10 @@ __global__ void __launch_bounds__(256) linear_int8_plain(const LiParams p) {
 // The weights' first stages are asked into L2 before the kernel in front has finished (programmatic dependent launch); nothing is read
 // into the block before that: the kernel in front may be the one that makes the weights.
 //
-// Waits are bounded: one that runs out records ULLM_STATUS_TIMEOUT, the block stores nothing, still meets its cluster, waits (bounded)
-// for its own copies in flight, frees its tensor memory and returns.
+// Waits for a barrier in shared memory are bounded: one that runs out records ULLM_STATUS_TIMEOUT, the block stores none of the results that
+// it waited for (of a shared tile none of the blocks does: the others are told between the cluster's two meetings), waits (bounded) for
+// its own copies in flight, frees its tensor memory and returns.  A cluster's meetings and the allocation of tensor memory have no limit of
+// their own: they end because every block comes to its meetings and to its release, whatever its waits did.
 // ---------------------------------------------------------------------------------------------
 #define LI_THREADS 192
 #define LI_W_BYTES (128 * 128)
@@ -285,6 +287,8 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
     // tokens that a block finishes, a multiple of 4: the sums travel as [block they come from][quad of tokens][channel][4 tokens]
     const int share = ((tokens + p.ksplit - 1) / p.ksplit + 3) & ~3;
     li_cluster_sync();  // every block's ring is drained (its accumulator is complete) or given up
+    if (warp == 2 && abort_flag && lane < p.ksplit)
+      asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(li_rank_addr(lin_smem(&abort_flag), lane)), "r"(1) : "memory");
     if (warp >= 2 && ok) {
       const uint32_t mine = lin_smem(ring) + (uint32_t)((rank * (share >> 2)) * 128 + chan) * 16;
       int to = 0, at = 0;  // the block that the next quad goes to, the quad's place there
@@ -303,7 +307,7 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
       }
     }
     li_cluster_sync();
-    if (warp >= 2 && ok && n < p.N) {
+    if (warp >= 2 && !abort_flag && n < p.N) {  // (set in any block of the cluster: some of the sums are missing)
       constexpr int W = NT < 32 ? 4 : 16;  // tokens at a time: their loads run beside one another
       const int4* got = reinterpret_cast<const int4*>(ring) + chan;
       const int mine_end = min(share, tokens - rank * share);
