@@ -38,7 +38,7 @@ def room(rows, cols, pad=0):
 # columns: one; less than a thread's piece; ragged; every number of pieces in registers; rows that are read twice
 SIZES = [(1, 1, 0), (3, 7, 0), (5, 64, 16), (2, 100, 28), (33, 1000, 0), (7, 2043, 5), (4, 4096, 0), (9, 8200, 8), (3, 12288, 0),
          (2, 20000, 16), (2, 33000, 8), (3, 40001, 0), (700, 128, 0),
-         # many rows: blocks that take one after the other, of one warp and of up to 32, with two and four rows on their way
+         # many rows, some of which blocks that stay take (32-bit ones; every form: test_gpu_int8_row_forms.py)
          (700, 1024, 0), (2500, 1032, 16), (301, 4096, 0), (640, 12288, 0), (900, 8200, 8), (300, 25600, 0), (299, 16384, 0), (310, 2047, 0)]
 
 

@@ -546,76 +546,110 @@ __global__ void __launch_bounds__(1024) rows_int8_stream(const RqParams p) {
 
 static int g_rq_sms = 0;
 
-// True where rows_int8_stream takes the rows (`code` is then the launch's): many and long ones.  us there and below: 2,048 x 25,600 gated
-// 53.7 and 75.7, 2,048 x 16,384 plain 18.8 and 25.9, 1,000 11.7 and 14.3, 300 6.6 and 6.1; 2,048 x 8,192 plain 11.8 and 12.2, gated 19.6
-// and 19.4.  A norm reads its weight beside the rows and is never faster there (2,048 x 4,096 14.2 and 13.0).
-template <typename T, int KIND>
-static bool rq_try_stream(const RqParams& p, int rows, cudaStream_t st, int* code) {
-  constexpr int VEC = 16 / (int)sizeof(T);
-  if (g_rq_sms == 0) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&g_rq_sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-      return false;
-  }
-  const int groups = p.cols / VEC, threads = ((groups + 3) / 4 + 31) / 32 * 32;
-  const long long slot = ((long long)p.cols * sizeof(T) * (KIND == RQ_ACT ? 2 : 1) + 127) / 128 * 128;
-  if (rows < 4 * g_rq_sms || groups < 2048 || groups > 4096 || RQ_SLOTS * slot > 208 * 1024) return false;
-  const int smem = (int)(RQ_SLOTS * slot);
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(rows_int8_stream<T, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024) != cudaSuccess)
-      return *code = ULLM_ERR_LAUNCH, true;
-    set = true;
-  }
-  int per_sm = 216 * 1024 / (smem + 2048);
-  if (per_sm > 1088 / threads) per_sm = 1088 / threads;  // (60 registers a thread)
-  if (per_sm < 1) per_sm = 1;
-  const int most = per_sm * g_rq_sms, each = (rows + most - 1) / most;  // (every block the same number of rows, or one less)
-  *code = ullm_launch_kernel(rows_int8_stream<T, KIND>, dim3((rows + each - 1) / each), dim3(threads), smem, st, p);
-  return true;
-}
+// The form that rows take: blocks that stay (`stream`), or a block a row with `per` groups of `vec` elements a thread (0: read twice), at any
+// address (`any`).
+struct RqForm {
+  bool stream, any;
+  int vec, per;
+};
 
 // Groups of a thread.  One, where a row's groups are threads enough: 2,048 x 4,096 normed 13.0 us, with two 15.2; rows as they are are
 // less work and take two from 256 groups on (2,048 x 4,096 6.7 for 8.0, 8 x 8,192 1.61 for 1.69).  Element by element many rows take two
 // from 384 on (1,000 x 531 normed 3.3, with one 4.8) and four from 768 (8-bit rows anywhere: 1,000 x 2,043 9.7, with two 11.7, with eight
 // 13.3).
-template <typename T, int KIND, int VEC, bool ANY = false>
-static int rq_launch_vec(const RqParams& p, int rows, cudaStream_t st) {
-  const int groups = (p.cols + VEC - 1) / VEC;
-  auto go = [&](auto kernel, int per) {
-    int threads = ((groups + per - 1) / per + 31) / 32 * 32;
-    return ullm_launch_kernel(kernel, dim3(rows), dim3(threads > 1024 ? 1024 : threads), 0, st, p);
-  };
-  const int least = VEC == 1 ? (rows <= 256 || groups < 384 ? 1 : groups < 768 ? 2 : 4) : KIND == RQ_PLAIN && groups >= 256 ? 2 : 1;
-  if constexpr (VEC == 1) {
-    if (groups > 4096 && groups <= 8192) return go(rows_int8_kernel<T, KIND, VEC, 8>, 8);
+static RqForm rq_block_form(int kind, int vec, bool any, int rows, int cols) {
+  const int groups = (cols + vec - 1) / vec;
+  const int least = vec == 1 ? (rows <= 256 || groups < 384 ? 1 : groups < 768 ? 2 : 4) : kind == RQ_PLAIN && groups >= 256 ? 2 : 1;
+  const int per = vec == 1 && groups > 4096 && groups <= 8192 ? 8
+                  : groups <= 1024 && least < 2               ? 1
+                  : groups <= 2048 && least < 3               ? 2
+                  : groups <= 4096                            ? 4
+                                                              : 0;
+  return {false, any, vec, per};
+}
+
+// `wide`: 16-byte pieces of every input row, V bytes of every output row; `borders`: of the weight and the output alone.
+static RqForm rq_choose(int kind, int element, int rows, int cols, bool wide, bool borders) {
+  const int V = 16 / element, groups = cols / V;
+  // Blocks that stay take many and long rows.  us there and below: 2,048 x 25,600 gated 53.7 and 75.7, 2,048 x 16,384 plain 18.8 and 25.9,
+  // 1,000 11.7 and 14.3, 300 6.6 and 6.1; 2,048 x 8,192 plain 11.8 and 12.2, gated 19.6 and 19.4.  A norm reads its weight beside the rows
+  // and is never faster there (2,048 x 4,096 14.2 and 13.0).
+  const long long slot = ((long long)cols * element * (kind == RQ_ACT ? 2 : 1) + 127) / 128 * 128;
+  if (kind != RQ_NORM && wide && rows >= 4 * g_rq_sms && groups >= 2048 && groups <= 4096 && RQ_SLOTS * slot <= 208 * 1024)
+    return {true, false, V, 4};
+  if (wide) return rq_block_form(kind, V, false, rows, cols);
+  // Pieces that are shifted into place cost little rows a longer way (the ends' elements come one by one) and many rows less work.  us so
+  // and element by element, normed, bfloat16: 1 x 4,091 2.8 and 2.9, 1 x 1,003 2.7 and 1.8; 64 x 2,043 3.0 and 3.0, 300 x 1,003 3.2 and 3.5,
+  // 1,000 x 531 5.0 and 3.3, 2,048 x 531 5.8 and 6.4; 2,048 x 4,091 22.8 and 34.4.  Plain 2,048 x 8,001 16.4 and 42.6, gated 2,048 x 9,001
+  // 35.6 and 67.2.
+  const long long n = (long long)rows * cols;
+  const bool many = cols >= 4000 || (cols >= 1000 && n >= 1 << 17) || (cols >= 500 && n >= 1 << 20);
+  if (many && borders && cols <= 4096 * V) return rq_block_form(kind, V, true, rows, cols);
+  return rq_block_form(kind, 1, false, rows, cols);
+}
+
+template <typename T, int KIND>
+static int rq_launch_stream(const RqParams& p, int rows, cudaStream_t st) {
+  const int groups = p.cols / (16 / (int)sizeof(T)), threads = ((groups + 3) / 4 + 31) / 32 * 32;
+  const long long slot = ((long long)p.cols * sizeof(T) * (KIND == RQ_ACT ? 2 : 1) + 127) / 128 * 128;
+  const int smem = (int)(RQ_SLOTS * slot);
+  static bool set = false;
+  if (!set) {
+    if (cudaFuncSetAttribute(rows_int8_stream<T, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024) != cudaSuccess)
+      return ULLM_ERR_LAUNCH;
+    set = true;
   }
-  if (groups <= 1024 && least < 2) return go(rows_int8_kernel<T, KIND, VEC, 1, ANY>, 1);
-  if (groups <= 2048 && least < 3) return go(rows_int8_kernel<T, KIND, VEC, 2, ANY>, 2);
-  if (groups <= 4096) return go(rows_int8_kernel<T, KIND, VEC, 4, ANY>, 4);
-  return go(rows_int8_kernel<T, KIND, VEC, 0>, 4);
+  int per_sm = 216 * 1024 / (smem + 2048);
+  if (per_sm > 1024 / threads) per_sm = 1024 / threads;  // (up to 64 registers a thread)
+  if (per_sm < 1) per_sm = 1;
+  const int most = per_sm * g_rq_sms, each = (rows + most - 1) / most;  // (every block the same number of rows, or one less)
+  return ullm_launch_kernel(rows_int8_stream<T, KIND>, dim3((rows + each - 1) / each), dim3(threads), smem, st, p);
+}
+
+template <typename T, int KIND, int VEC, bool ANY>
+static int rq_launch_block(const RqParams& p, int rows, int per, cudaStream_t st) {
+  const int groups = (p.cols + VEC - 1) / VEC, each = per > 0 ? per : 4, threads = ((groups + each - 1) / each + 31) / 32 * 32;
+  auto go = [&](auto kernel) { return ullm_launch_kernel(kernel, dim3(rows), dim3(threads > 1024 ? 1024 : threads), 0, st, p); };
+  if (per == 1) return go(rows_int8_kernel<T, KIND, VEC, 1, ANY>);
+  if (per == 2) return go(rows_int8_kernel<T, KIND, VEC, 2, ANY>);
+  if (per == 4) return go(rows_int8_kernel<T, KIND, VEC, 4, ANY>);
+  if constexpr (VEC == 1) {
+    if (per == 8) return go(rows_int8_kernel<T, KIND, VEC, 8, ANY>);
+  }
+  if constexpr (!ANY) return go(rows_int8_kernel<T, KIND, VEC, 0, ANY>);
+  return ULLM_ERR_UNSUPPORTED;
+}
+
+static bool rq_read_sms() {
+  int dev = 0;
+  if (g_rq_sms == 0 && (cudaGetDevice(&dev) != cudaSuccess ||
+                        cudaDeviceGetAttribute(&g_rq_sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess))
+    g_rq_sms = 0;
+  return g_rq_sms > 0;
 }
 
 template <typename T, int KIND>
 static int rq_launch(const RqParams& p, int rows, cudaStream_t st) {
   constexpr int V = 16 / (int)sizeof(T);
-  // 16-byte pieces of every input row, V bytes of every output row
-  const bool wide = p.cols % V == 0 && (uintptr_t)p.x % 16 == 0 && p.x_stride % V == 0 && (uintptr_t)p.residual % 16 == 0 &&
-                    (uintptr_t)p.weight % 16 == 0 && (uintptr_t)p.out % V == 0 && p.out_stride % V == 0;
-  int code = ULLM_OK;
-  if constexpr (KIND != RQ_NORM) {
-    if (wide && rq_try_stream<T, KIND>(p, rows, st, &code)) return code;
-  }
-  if (wide) return rq_launch_vec<T, KIND, V>(p, rows, st);
-  // Pieces that are shifted into place cost little rows a longer way (the ends' elements come one by one) and many rows less work.  us so
-  // and element by element, normed, bfloat16: 1 x 4,091 2.8 and 2.9, 1 x 1,003 2.7 and 1.8; 64 x 2,043 3.0 and 3.0, 300 x 1,003 3.2 and 3.5,
-  // 1,000 x 531 5.0 and 3.3, 2,048 x 531 5.8 and 6.4; 2,048 x 4,091 22.8 and 34.4.  Plain 2,048 x 8,001 16.4 and 42.6, gated 2,048 x 9,001
-  // 35.6 and 67.2.
-  const long long n = (long long)rows * p.cols;
-  const bool many = p.cols >= 4000 || (p.cols >= 1000 && n >= 1 << 17) || (p.cols >= 500 && n >= 1 << 20);
   const bool borders = (uintptr_t)p.weight % 16 == 0 && (uintptr_t)p.out % V == 0 && p.out_stride % V == 0;
-  if (many && borders && p.cols <= 4096 * V) return rq_launch_vec<T, KIND, V, true>(p, rows, st);
-  return rq_launch_vec<T, KIND, 1>(p, rows, st);
+  const bool wide = borders && p.cols % V == 0 && (uintptr_t)p.x % 16 == 0 && p.x_stride % V == 0 && (uintptr_t)p.residual % 16 == 0;
+  if (!rq_read_sms()) return ULLM_ERR_LAUNCH;
+  const RqForm f = rq_choose(KIND, sizeof(T), rows, p.cols, wide, borders);
+  if constexpr (KIND != RQ_NORM) {
+    if (f.stream) return rq_launch_stream<T, KIND>(p, rows, st);
+  }
+  if (f.any) return rq_launch_block<T, KIND, V, true>(p, rows, f.per, st);
+  if (f.vec == V) return rq_launch_block<T, KIND, V, false>(p, rows, f.per, st);
+  return rq_launch_block<T, KIND, 1, false>(p, rows, f.per, st);
+}
+
+// The form that such rows take: -1 blocks that stay, else 100 * elements of a group + groups of a thread (0: read twice), 1,000 more for rows at
+// any address; 0 for sizes that no call takes.  kind: 0 as they are, 1 gated, 2 normed; place: 2 all rows come in pieces of 16 bytes, 1 the
+// weight and the output alone lie on borders, 0 nothing does.
+extern "C" int ullm_rows_int8_form(int kind, int dtype, int rows, int cols, int place) {
+  if (kind < RQ_PLAIN || kind > RQ_NORM || rows <= 0 || cols <= 0 || !rq_read_sms()) return 0;
+  const RqForm f = rq_choose(kind, dtype == ULLM_DTYPE_F32 ? 4 : 2, rows, cols, place == 2, place > 0);
+  return f.stream ? -1 : 1000 * f.any + 100 * f.vec + f.per;
 }
 
 template <int KIND>
