@@ -5,7 +5,7 @@ import torch
 
 from conftest import device
 from plain_int8 import check_rows, gated, normed
-from test_gpu_int8 import gen, room, rows_of
+from test_gpu_int8 import gen, placed, room, rows_of
 from test_gpu_kernels import K
 
 pytestmark = [pytest.mark.gpu, pytest.mark.needs_cuda]
@@ -86,4 +86,20 @@ def test_rows_of_every_form(rows, cols, place, dtype):
     K().add_rmsnorm_int8(x, res, weight, 1e-6, q, scales)
     check_rows(q, scales, y, 2.0 ** -23, 2.0 ** -24 * ((cols / 1024 + 40) / 2 + 10))
     assert torch.equal(res, want)
+    untouched()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols,offset", [(9, 4096, 0), (2, 16384, 0), (2, 33024, 0), (2, 40001, 0), (9, 1003, 3), (9, 4091, 0), (5, 9001, 1),
+                                              (3, 16387, 5), (300, 2043, 2)])
+def test_a_residual_that_is_the_input_in_every_form(rows, cols, offset, dtype):
+    """x and residual one tensor: in registers, read twice, element by element, and in pieces whose stores take a neighbour's elements along."""
+    once, weight = rows_of(gen(cols), rows, cols, dtype), torch.ones(cols, device=device())
+    x, around = placed(once, offset)
+    q, untouched = room(rows, cols, -cols % 16)
+    scales = torch.empty(rows, device=device())
+    K().add_rmsnorm_int8(x, x, weight, 1e-6, q, scales)
+    check_rows(q, scales, normed(once, once, weight, 1e-6), 2.0 ** -23, 2.0 ** -24 * ((cols / 1024 + 40) / 2 + 10))
+    assert torch.equal(x, (once.float() * 2).to(dtype))
+    around()
     untouched()
