@@ -2,8 +2,8 @@
 // per token (row of x) and per channel (row of w); out in float32, bfloat16 or float16.
 //
 // The sum is a whole number in 32 bits and exact: |sum| <= 2^14 K < 2^31 for K <= 131,071, whatever the order of its terms, so that how
-// a product is cut does not show in its result.  The result is formed in float32, times x_scales first, and rounded once.  A token whose
-// scale is NaN (a row that had no finite maximum) has NaN results; no other token's change.
+// a product is cut does not show in its result.  The result is formed in float32, times x_scales first (beyond 2^96 last), and rounded
+// once.  A token whose scale is NaN (a row that had no finite maximum) has NaN results; no other token's change.
 //
 // Three kernels:
 //   linear_int8_tc      the tcgen05 tensor cores (kind::i8), operands by TMA (rows on borders of 16 bytes): few tokens, narrow products;
@@ -33,17 +33,25 @@ template <typename T>
 __device__ __forceinline__ T li_result(int sum, float xs, float ws, float bias) {
   return from_f32<T>(fmaf((float)sum * xs, ws, bias));
 }
+// A sum times an x_scale beyond 2^96 may pass what 32 bits hold, where the result does not: such tokens meet the other scale first.
+__device__ __forceinline__ bool li_large(float xs) { return fabsf(xs) > 7.922816251426434e28f; }
 
 // One channel of W tokens, of which `tokens` exist: out[i * stride] = result of v[i].  All scales are read before the first store,
 // which the compiler could not move them in front of (out might be anywhere): 64 columns end in 0.6 us instead of 2.
-template <typename T, int W>
-__device__ __forceinline__ void li_store(T* out, int stride, const int (&v)[W], const float* xs, float ws, float bias, int tokens) {
+template <typename T, int W, bool LARGE>
+__device__ __forceinline__ void li_store_some(T* out, int stride, const int (&v)[W], const float* xs, float ws, float bias, int tokens) {
   T r[W];
 #pragma unroll
   for (int i = 0; i < W; i += 4) {
     const float4 s = *reinterpret_cast<const float4*>(xs + i);
     r[i] = li_result<T>(v[i], s.x, ws, bias), r[i + 1] = li_result<T>(v[i + 1], s.y, ws, bias);
     r[i + 2] = li_result<T>(v[i + 2], s.z, ws, bias), r[i + 3] = li_result<T>(v[i + 3], s.w, ws, bias);
+    if constexpr (LARGE) {
+      const float e[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (li_large(e[j])) r[i + j] = li_result<T>(v[i + j], ws, e[j], bias);
+    }
   }
   if (tokens >= W) {
 #pragma unroll
@@ -53,6 +61,22 @@ __device__ __forceinline__ void li_store(T* out, int stride, const int (&v)[W], 
     for (int i = 0; i < W; ++i, out += stride)
       if (i < tokens) *out = r[i];
   }
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void li_store(bool large, T* out, int stride, const int (&v)[W], const float* xs, float ws, float bias, int tokens) {
+  if (large) li_store_some<T, W, true>(out, stride, v, xs, ws, bias, tokens);
+  else li_store_some<T, W, false>(out, stride, v, xs, ws, bias, tokens);
+}
+// The meeting of the 128 finishing threads (barrier 1): whether one of them says so.
+__device__ __forceinline__ bool li_meet(bool mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(any)
+      : "r"((uint32_t)mine)
+      : "memory");
+  return any != 0;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -95,7 +119,11 @@ __global__ void __launch_bounds__(256) linear_int8_plain(const LiParams p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const long long m = m0 + tm + 8 * i;
-      if (m < p.M && n < p.N) reinterpret_cast<T*>(p.out)[m * p.N + n] = li_result<T>(acc[i], p.x_scales[m], ws_n, bias);
+      if (m < p.M && n < p.N) {
+        const float xs_m = p.x_scales[m];
+        const bool large = li_large(xs_m);
+        reinterpret_cast<T*>(p.out)[m * p.N + n] = li_result<T>(acc[i], large ? ws_n : xs_m, large ? xs_m : ws_n, bias);
+      }
     }
   }
 }
@@ -265,9 +293,13 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
   T* out = reinterpret_cast<T*>(p.out);
   const float ws = warp >= 2 && n < p.N ? p.w_scales[n] : 0.f;
   const float bias = warp >= 2 && n < p.N && p.bias != nullptr ? to_f32(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
+  bool large = false;  // whether one of the tile's tokens is
   if (warp >= 2) {
-    for (int i = threadIdx.x - 64; i < tokens; i += 128) xs_s[i] = p.x_scales[m0 + i];
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    for (int i = threadIdx.x - 64; i < tokens; i += 128) {
+      const float xs = xs_s[i] = p.x_scales[m0 + i];
+      large |= li_large(xs);
+    }
+    large = li_meet(large);
     ok = __all_sync(0xffffffffu, mbar_wait(&acc_bar, 0));
     if (!ok) {
       if (lane == 0) ullm_report(p.status, ULLM_STATUS_TIMEOUT, 133, 0);
@@ -280,7 +312,7 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
       for (int c = 0; c < tokens; c += 16) {
         int v[16];
         li_tmem_ld16(taddr + c, v);
-        if (n < p.N) li_store<T, 16>(out + (size_t)(m0 + c) * p.N + n, p.N, v, xs_s + c, ws, bias, tokens - c);
+        if (n < p.N) li_store<T, 16>(large, out + (size_t)(m0 + c) * p.N + n, p.N, v, xs_s + c, ws, bias, tokens - c);
       }
     }
   } else {
@@ -324,7 +356,7 @@ __global__ void __launch_bounds__(LI_THREADS) linear_int8_tc(const __grid_consta
           }
         }
         const int m = rank * share + t;
-        li_store<T, W>(out + (size_t)(m0 + m) * p.N + n, p.N, v, xs_s + m, ws, bias, mine_end - t);
+        li_store<T, W>(large, out + (size_t)(m0 + m) * p.N + n, p.N, v, xs_s + m, ws, bias, mine_end - t);
       }
     }
   }
@@ -523,7 +555,11 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
       const int buf = it & 1;
       const int n = (int)(tile / t_tiles) * 256 + rank * 128 + quarter * 32 + lane, m0 = (int)(tile % t_tiles) * BN;
       const int tokens = min(BN, p.M - m0);
-      for (int i = threadIdx.x - 64; i < BN; i += 128) xs_s[buf][i] = i < tokens ? p.x_scales[m0 + i] : 0.f;
+      bool large = false;  // whether one of the tile's tokens is
+      for (int i = threadIdx.x - 64; i < BN; i += 128) {
+        const float xs = xs_s[buf][i] = i < tokens ? p.x_scales[m0 + i] : 0.f;
+        large |= li_large(xs);
+      }
       const float ws = n < p.N ? p.w_scales[n] : 0.f;
       const float bias = n < p.N && p.bias != nullptr ? to_f32(reinterpret_cast<const T*>(p.bias)[n]) : 0.f;
       // one thread waits (bounded) and tells the others, so that all 128 take the same way out
@@ -532,7 +568,7 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
         if (!got) ullm_report(p.status, ULLM_STATUS_TIMEOUT, 137, it), abort_flag = 1;
         go[buf] = got;
       }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      large = li_meet(large);
       if (!go[buf]) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t taddr = tmem_d + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN);
@@ -540,7 +576,7 @@ linear_int8_pair(const __grid_constant__ CUtensorMap w_map, const __grid_constan
       for (int c = 0; c < tokens; c += 32) {
         int v[32];
         li_tmem_ld32(taddr + c, v);
-        if (n < p.N) li_store<T, 32>(out + (size_t)c * p.N, p.N, v, xs_s[buf] + c, ws, bias, tokens - c);
+        if (n < p.N) li_store<T, 32>(large, out + (size_t)c * p.N, p.N, v, xs_s[buf] + c, ws, bias, tokens - c);
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
