@@ -367,16 +367,37 @@ __device__ __forceinline__ void rq_store(const RqRow& r, signed char* out, const
 
 // A gated row in which the elements beyond the fast gate may count, by the whole block, two reads of the row x [gate | up].  They are up to
 // 2^-119 |up| each: below half a step, and so nothing, where the row's largest is not below 2^-20 and no up above 2^91.  (Looking for
-// such ups would cost every row: 16 x 12,288 2.64 us and 2.80.  Beside one, a gate that far below zero counts as zero.)
-template <typename T>
+// such ups would cost every row: 16 x 12,288 2.64 us and 2.80.  Beside one, a gate that far below zero counts as zero.)  Rows of zeros come
+// here too: 2,048 x 12,288 of them 52 us, of small rows 65, of others 28.
+// (VEC 4 or 1 at a time: with eight the whole kernel would take more than 40 registers, and two blocks of 768 threads no longer find room.)
+template <typename T, int VEC>
+__device__ __forceinline__ void rq_load_far(const T* x, int cols, int act, int c, float (&v)[VEC]) {
+  struct alignas(VEC * sizeof(T)) Piece {
+    T e[VEC];
+  };
+  const Piece g = *reinterpret_cast<const Piece*>(x + c), up = *reinterpret_cast<const Piece*>(x + cols + c);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = rq_gate_times(to_f32(g.e[i]), to_f32(up.e[i]), act);
+}
+template <typename T, int VEC>
 __device__ __noinline__ void rq_act_again(const T* x, signed char* out, float* scale, int cols, int act) {
-  float none = 0.f, most = 0.f;
-  for (int c = threadIdx.x; c < cols; c += blockDim.x) most = rq_max(most, rq_gate_times(to_f32(x[c]), to_f32(x[cols + c]), act));
+  float none = 0.f, most = 0.f, v[VEC];
+#pragma unroll 1
+  for (int c = threadIdx.x * VEC; c < cols; c += blockDim.x * VEC) {
+    rq_load_far<T, VEC>(x, cols, act, c, v);
+    most = rq_most<VEC>(most, v);
+  }
   const RqRow r = rq_row<T, RQ_ACT>(rq_reduce(none, most, false));
   if (threadIdx.x == 0) *scale = rq_scale(r);
-  for (int c = threadIdx.x; c < cols; c += blockDim.x) {
-    const float v[1] = {rq_gate_times(to_f32(x[c]), to_f32(x[cols + c]), act)};
-    rq_store<false, 1>(r, out + c, v);
+#pragma unroll 1
+  for (int c = threadIdx.x * VEC; c < cols; c += blockDim.x * VEC) {
+    if (r.most == 0.f) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = 0.f;
+    } else {
+      rq_load_far<T, VEC>(x, cols, act, c, v);
+    }
+    rq_store<false, VEC>(r, out + c, v);
   }
 }
 template <int KIND>
@@ -448,7 +469,7 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RqParams p) {
   }
   const uint32_t top = rq_join<KIND>(p, sum, most);
   if constexpr (KIND == RQ_ACT) {
-    if (rq_is_far<KIND>(top)) return rq_act_again(x, out, p.scales + row, p.cols, p.act);
+    if (rq_is_far<KIND>(top)) return rq_act_again<T, ANY || VEC < 4 ? 1 : 4>(x, out, p.scales + row, p.cols, p.act);
   }
   const RqRow r = rq_row<T, KIND>(top);
   if (threadIdx.x == 0)
@@ -529,7 +550,7 @@ __global__ void __launch_bounds__(1024) rows_int8_stream(const RqParams p) {
     }
     signed char* out = p.out + row * p.out_stride;
     if (KIND == RQ_ACT && rq_is_far<KIND>(top)) {
-      rq_act_again(reinterpret_cast<const T*>(p.x) + row * p.x_stride, out, p.scales + row, p.cols, p.act);
+      rq_act_again<T, 4>(reinterpret_cast<const T*>(p.x) + row * p.x_stride, out, p.scales + row, p.cols, p.act);
     } else {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
