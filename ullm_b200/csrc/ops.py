@@ -844,7 +844,8 @@ class Kernels:
 
     def add_rmsnorm_int8(self, x, residual, weight, eps: float, out, scales):
         """`add_rmsnorm` with its result in 8 bits: s = x + residual in 32-bit, residual <- s rounded (in place; residual may be None),
-        out (int8 [T, C]), scales (float32 [T]) <- the rows s / sqrt(mean(s^2) + eps) * weight."""
+        out (int8 [T, C]), scales (float32 [T]) <- the rows s / sqrt(mean(s^2) + eps) * weight.  (Rows of any size whose s * weight
+        32 bits hold.)"""
         if self._unwatched() and _at_once.add_rmsnorm_int8(self.lib.ullm_add_rmsnorm_int8, x, residual, weight, eps, out, scales,
                                                            self.status) == 0:
             self.launches += 1

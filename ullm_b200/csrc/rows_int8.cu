@@ -27,10 +27,10 @@
 // The work is bound by memory.  Two forms:
 //   rows_int8_kernel   a block takes one row and holds it in registers between the reduction and the store (PER groups of VEC
 //                      neighbouring elements per thread, all loads in flight together); rows too long for that are read a second
-//                      time.  Few rows, and rows that do not come in pieces of 16 bytes: pieces shifted into place, or element by
+//                      time.  Norms, few rows, and rows that do not come in pieces of 16 bytes: pieces shifted into place, or element by
 //                      element.
 //   rows_int8_stream   blocks that stay and take one row after the other, the next rows on their way into shared memory (bulk copies)
-//                      while one is worked on.  Many rows.
+//                      while one is worked on.  Many long rows as they are and gated (`rq_choose`); norms never.
 #include <type_traits>
 
 #include "tcgen05_util.cuh"
@@ -601,7 +601,7 @@ static RqForm rq_choose(int kind, int element, int rows, int cols, bool wide, bo
   if (wide) return rq_block_form(kind, V, false, rows, cols);
   // Pieces that are shifted into place cost little rows a longer way (the ends' elements come one by one) and many rows less work.  us so
   // and element by element, normed, bfloat16: 1 x 4,091 2.8 and 2.9, 1 x 1,003 2.7 and 1.8; 64 x 2,043 3.0 and 3.0, 300 x 1,003 3.2 and 3.5,
-  // 1,000 x 531 5.0 and 3.3, 2,048 x 531 5.8 and 6.4; 2,048 x 4,091 22.8 and 34.4.  Plain 2,048 x 8,001 16.4 and 42.6, gated 2,048 x 9,001
+  // 1,000 x 531 5.0 and 3.3, 2,048 x 531 5.8 and 6.4; 2,048 x 4,091 21.4 and 34.4.  Plain 2,048 x 8,001 16.4 and 42.6, gated 2,048 x 9,001
   // 35.6 and 67.2.
   const long long n = (long long)rows * cols;
   const bool many = cols >= 4000 || (cols >= 1000 && n >= 1 << 17) || (cols >= 500 && n >= 1 << 20);
